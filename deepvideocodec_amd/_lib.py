@@ -51,7 +51,22 @@ class DvcConv2d(C.Structure):
     ]
 
 
+CKPT_FORMATS = {"int8": 0, "e4m3": 1}
+MAX_TOP = 16
+
+
+class DvcCkpt(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("channels", C.c_int32), ("format", C.c_int32)]
+
+
+class DvcLogits(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("batch_stride", C.c_int64), ("class_stride", C.c_int64),
+                ("groups", C.c_int32), ("classes", C.c_int32), ("dtype", C.c_int32), ("_pad", C.c_int32)]
+
+
 _P = C.c_void_p
+_CK = C.POINTER(DvcCkpt)
+_LG = C.POINTER(DvcLogits)
 _SRC = C.POINTER(DvcSrc)
 _DST = C.POINTER(DvcDst)
 _i32, _i64, _f32 = C.c_int32, C.c_int64, C.c_float
@@ -110,6 +125,16 @@ SIGNATURES = {
                                                 _i32, _i32, _i32, _P]),
     "dvc_likelihood_bits_backward": (C.c_int, [_SRC, _P, _DST, _i32, _i32, _i32, _P]),
     "dvc_sq_err_backward": (C.c_int, [_SRC, _SRC, _P, _DST, _i32, _i32, _i32, _P]),
+    "dvc_act_checkpoint": (C.c_int, [_SRC, _i32, _f32, _i32, _P, _P, _i32, _i32, _i32, _P]),
+    "dvc_act_restore": (C.c_int, [_CK, _DST, _i32, _i32, _i32, _P]),
+    "dvc_act_signs": (C.c_int, [_SRC, _P, _i32, _i32, _i32, _P]),
+    "dvc_act_grad_signs": (C.c_int, [_SRC, _P, _f32, _i32, _P, _i32, _i32, _i32, _i32, _P]),
+    "dvc_mul_act_grad_ckpt": (C.c_int, [_SRC, _CK, _f32, _SRC, _DST, _i32, _i32, _i32, _P]),
+    "dvc_conv2d_wgrad_ckpt_scratch_floats": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "dvc_conv2d_wgrad_ckpt": (C.c_int, [_CK, _i32, _i32, _i32, _i32, _P, _i32, _i32, _i32, _P, _P, _P, _P]),
+    "dvc_symbol_log_probs_scratch_floats": (_i64, [_LG, _i32, _i32, _i32, _i32]),
+    "dvc_symbol_log_probs": (C.c_int, [_LG, _P, _i32, _P, _P, _P, _P, _P, _P, _i32, _i32, _i32, _P]),
+    "dvc_symbol_log_probs_backward": (C.c_int, [_LG, _P, _P, _P, _P, _P, _P, _i32, _i32, _i32, _P]),
     "dvc_rans_encode": (_i64, [_P, _P, _i64, _P, _i32, _i32, _P, _P, _P, _i64]),
     "dvc_rans_decode": (C.c_int, [_P, _i64, _P, _i64, _P, _i32, _i32, _P, _P, _P]),
     "dvc_pmf_to_quantized_cdf": (C.c_int, [_P, _i32, _i32, _P]),

@@ -30,7 +30,7 @@ class _Conv2d(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, weight, bias, stride, in_slope, out_slope, pixel_shuffle, packed, dgrad_packed, precision,
-                dgrad_precision, residual, residual2, *srcs):
+                dgrad_precision, storage, residual, residual2, *srcs):
         # (residual operands only for a layer without output activation: the sum's adjoint is then the identity on
         # every operand and needs nothing saved; see conv2d() below)
         out = ops.conv2d(srcs, weight, bias, stride=stride, in_slope=in_slope, out_slope=out_slope,
@@ -39,13 +39,22 @@ class _Conv2d(torch.autograd.Function):
         ctx.cfg = (stride, in_slope, out_slope, pixel_shuffle, bias is not None)
         ctx.dgrad_packed = dgrad_packed     # the layer's cached data-gradient weight image (or None: packed on demand)
         ctx.dgrad_precision = dgrad_precision
-        ctx.save_for_backward(weight, out if out_slope is not None else None, *srcs)
+        if storage is None:
+            ctx.kept = None
+            ctx.save_for_backward(weight, out if out_slope is not None else None, *srcs)
+        else:
+            # 8-bit storage: the activated sources as checkpoints (for the weight gradient and, by their sign bits, the
+            # input activation's derivative), the output activation's derivative as one bit per value
+            ctx.kept, tensors = _keep(srcs, in_slope, storage, ctx.needs_input_grad[0] or in_slope is not None)
+            ctx.save_for_backward(weight, ops.act_signs(out) if out_slope is not None else None, *tensors)
         return out
 
     @staticmethod
     def backward(ctx, g):
         stride, in_slope, out_slope, ps, has_bias = ctx.cfg
         weight, out, *srcs = ctx.saved_tensors
+        if ctx.kept is not None:
+            srcs = _kept(ctx.kept, srcs)
         cout, cin, k, _ = weight.shape
         n, _, h, w = srcs[0].shape
         pad = k // 2
@@ -54,17 +63,17 @@ class _Conv2d(torch.autograd.Function):
         if out_slope is None and not ps and g.is_contiguous():
             g_pre = g
         else:
-            g_pre = ops.act_grad(g, out, 1.0 if out_slope is None else out_slope, ps, (n, cout, ho, wo))
+            g_pre = _act_grad(g, out, 1.0 if out_slope is None else out_slope, ps, (n, cout, ho, wo))
         need = ctx.needs_input_grad
         gw = gb = None
         if need[0] and has_bias and need[1]:     # the bias gradient rides along with the weight gradient
-            gw, gb = ops.conv2d_wgrad(srcs, g_pre, weight.shape, stride, in_slope, with_bias=True)
+            gw, gb = _wgrad(srcs, g_pre, weight.shape, stride, in_slope, True)
         elif need[0]:
-            gw = ops.conv2d_wgrad(srcs, g_pre, weight.shape, stride, in_slope)
+            gw = _wgrad(srcs, g_pre, weight.shape, stride, in_slope, False)
         elif has_bias and need[1]:
             gb = ops.plane_dot(g_pre, None, sum_batch=True)
         gsrcs = [None] * len(srcs)
-        if any(need[12:]):
+        if any(need[13:]):
             # data gradient = stride-1 convolution of (zero-upsampled) g_pre with the flipped,
             # transposed kernel -- the same MFMA kernel as the forward pass (and in the same operand mode)
             gin = ops.zero_upsample2(g_pre, h, w) if stride == 2 else g_pre
@@ -72,13 +81,52 @@ class _Conv2d(torch.autograd.Function):
             gx = ops.conv2d(gin, (cin, cout, k, k), None, stride=1, packed=image, precision=ctx.dgrad_precision)
             c0 = 0
             for i, s in enumerate(srcs):
-                c1 = c0 + s.size(1)
-                if need[12 + i]:
+                c1 = c0 + s.shape[1]
+                if need[13 + i]:
                     gs = gx[:, c0:c1]
-                    gsrcs[i] = ops.mul_act_grad(gs, s, in_slope) if in_slope is not None else gs
+                    gsrcs[i] = _mul_act_grad(gs, s, in_slope) if in_slope is not None else gs
                 c0 = c1
-        return (gw, gb, None, None, None, None, None, None, None, None, g if need[10] else None,
-                g if need[11] else None, *gsrcs)
+        return (gw, gb, None, None, None, None, None, None, None, None, None, g if need[11] else None,
+                g if need[12] else None, *gsrcs)
+
+
+class _ShapeOnly:
+    """A source whose values the backward pass does not need."""
+
+    def __init__(self, shape):
+        self.shape = shape
+
+
+def _keep(srcs, slope, fmt, values):
+    """8-bit checkpoints of LeakyReLU(slope)(srcs): (what _kept() needs besides the tensors, the tensors)."""
+    if not values:
+        return [(tuple(s.shape), None) for s in srcs], []
+    cks = [ops.act_checkpoint(s, slope, fmt) for s in srcs]
+    return [(ck.shape, ck.fmt) for ck in cks], [t for ck in cks for t in (ck.codes, ck.scales)]
+
+
+def _kept(kept, tensors):
+    return [_ShapeOnly(shape) if fmt is None else ops.ActCheckpoint(tensors[2 * i], tensors[2 * i + 1], shape, fmt)
+            for i, (shape, fmt) in enumerate(kept)]
+
+
+# the adjoints that read a stored activation, whichever way it was stored
+def _act_grad(g, out, slope, pixel_shuffle, conv_shape):
+    if out is not None and out.dtype == torch.int32:
+        return ops.act_grad_signs(g, out, slope, pixel_shuffle, conv_shape)
+    return ops.act_grad(g, out, slope, pixel_shuffle, conv_shape)
+
+
+def _mul_act_grad(g, x, slope, out=None, plus=None):
+    if isinstance(x, ops.ActCheckpoint):
+        return ops.mul_act_grad_ckpt(g, x, slope, out=out, plus=plus)
+    return ops.mul_act_grad(g, x, slope, out=out, plus=plus)
+
+
+def _wgrad(srcs, g_pre, wshape, stride, in_slope, with_bias):
+    if isinstance(srcs[0], ops.ActCheckpoint):     # (the activation was applied before storing)
+        return ops.conv2d_wgrad_ckpt(srcs, g_pre, tuple(wshape), stride, with_bias=with_bias)
+    return ops.conv2d_wgrad(srcs, g_pre, wshape, stride, in_slope, with_bias=with_bias)
 
 
 def dgrad_weight_image(weight: Tensor, precision: int = 0) -> Tensor:
@@ -90,22 +138,25 @@ def dgrad_weight_image(weight: Tensor, precision: int = 0) -> Tensor:
 
 
 def conv2d(srcs, weight, bias, stride=1, in_slope=None, out_slope=None, residual=None, res_scale=None,
-           residual2=None, pixel_shuffle=False, packed=None, dgrad_packed=None, precision=0, dgrad_precision=0):
+           residual2=None, pixel_shuffle=False, packed=None, dgrad_packed=None, precision=0, dgrad_precision=0,
+           storage=None):
     """Differentiable ops.conv2d.  Behind an output activation, or with a gate, the residual adds are taken out of the
     convolution epilogue (their adjoint needs the pre-residual activation) and run as add_scaled.  `precision` / `dgrad_precision`: operand
     mode (ops.PRECISIONS) of the forward and of the data-gradient convolution -- `packed` / `dgrad_packed` must be images
-    in those modes; the weight gradient is always formed in fp32."""
+    in those modes; the weight gradient is always formed in fp32.  `storage`: None keeps the tensors the backward pass
+    reads in fp32; "int8" / "e4m3" keeps the sources as 8-bit checkpoints and the output's signs as bits (the weight
+    gradient is then that of the stored sources; data and bias gradients are unchanged)."""
     if isinstance(srcs, torch.Tensor):
         srcs = (srcs,)
     if residual is not None and out_slope is None and res_scale is None and not pixel_shuffle:
         # no activation between the convolution and the sum (the second convolution of a ResBlock,
         # dmc/models/layers.py:75-81): the sum stays in the convolution's epilogue, as on the coding path
         return _Conv2d.apply(weight, bias, stride, in_slope, out_slope, pixel_shuffle, packed, dgrad_packed, precision,
-                             dgrad_precision, residual, residual2, *srcs)
+                             dgrad_precision, storage, residual, residual2, *srcs)
     y = _Conv2d.apply(weight, bias, stride, in_slope, out_slope, pixel_shuffle, packed, dgrad_packed, precision,
-                      dgrad_precision, None, None, *srcs)
+                      dgrad_precision, storage, None, None, *srcs)
     if residual is not None:
-        y = add_scaled(y, residual, res_scale, residual2)
+        y = add_scaled(y, residual, res_scale, residual2, storage)
     return y
 
 
@@ -118,7 +169,7 @@ class _ResBlock(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, plus, w1, b1, w2, b2, slope_in, slope_mid, slope_out, packed1, packed2, dpacked1, dpacked2,
-                pf1, pd1, pf2, pd2):
+                pf1, pd1, pf2, pd2, storage):
         t = ops.conv2d(x, w1, b1, in_slope=slope_in, out_slope=slope_mid, packed=packed1, precision=pf1)
         if slope_out is None:
             y = ops.conv2d(t, w2, b2, residual=x, residual2=plus, packed=packed2, precision=pf2)
@@ -128,14 +179,22 @@ class _ResBlock(torch.autograd.Function):
             y = ops.add_scaled(u, x, None, plus)
         ctx.cfg = (slope_in, slope_mid, slope_out, pd1, pd2)
         ctx.images = (dpacked1, dpacked2)
-        ctx.save_for_backward(x, t, u, w1, w2)
+        if storage is None:
+            ctx.kept = None
+            ctx.save_for_backward(w1, w2, u, x, t)
+        else:
+            kx, tx = _keep((x,), slope_in, storage, True)
+            kt, tt = _keep((t,), None, storage, True)
+            ctx.kept = kx + kt
+            ctx.save_for_backward(w1, w2, ops.act_signs(u) if u is not None else None, *tx, *tt)
         return y
 
     @staticmethod
     def backward(ctx, g):
         slope_in, slope_mid, slope_out, pd1, pd2 = ctx.cfg
         dpacked1, dpacked2 = ctx.images
-        x, t, u, w1, w2 = ctx.saved_tensors
+        w1, w2, u, *xt = ctx.saved_tensors
+        x, t = xt if ctx.kept is None else _kept(ctx.kept, xt)
         need = ctx.needs_input_grad
         n, ch, h, w = x.shape
         mid = w1.shape[0]
@@ -144,16 +203,19 @@ class _ResBlock(torch.autograd.Function):
         if slope_out is None and g.is_contiguous():
             g2 = g
         else:
-            g2 = ops.act_grad(g, u, 1.0 if slope_out is None else slope_out, False, (n, ch, h, w))
+            g2 = _act_grad(g, u, 1.0 if slope_out is None else slope_out, False, (n, ch, h, w))
         gw2 = gb2 = gw1 = gb1 = None
         if need[4] or need[5]:
-            gw2, gb2 = ops.conv2d_wgrad((t,), g2, w2.shape, 1, None, with_bias=True)
+            gw2, gb2 = _wgrad((t,), g2, w2.shape, 1, None, True)
         image2 = dpacked2 if dpacked2 is not None else dgrad_weight_image(w2, pd2)
         gt = ops.conv2d(g2, (mid, ch, 3, 3), None, stride=1, packed=image2, precision=pd2)
         # first convolution (its output activation is the block's middle one)
-        g1 = ops.act_grad(gt, t, slope_mid, False, (n, mid, h, w))
+        if isinstance(t, ops.ActCheckpoint):
+            g1 = ops.mul_act_grad_ckpt(gt, t, slope_mid, out=gt)
+        else:
+            g1 = ops.act_grad(gt, t, slope_mid, False, (n, mid, h, w))
         if need[2] or need[3]:
-            gw1, gb1 = ops.conv2d_wgrad((x,), g1, w1.shape, 1, slope_in, with_bias=True)
+            gw1, gb1 = _wgrad((x,), g1, w1.shape, 1, slope_in, True)
         gx = None
         if need[0]:
             image1 = dpacked1 if dpacked1 is not None else dgrad_weight_image(w1, pd1)
@@ -161,10 +223,10 @@ class _ResBlock(torch.autograd.Function):
                 gx = ops.conv2d(g1, (ch, mid, 3, 3), None, stride=1, packed=image1, precision=pd1, residual=g)
             else:
                 gx = ops.conv2d(g1, (ch, mid, 3, 3), None, stride=1, packed=image1, precision=pd1)
-                gx = ops.mul_act_grad(gx, x, slope_in, out=gx, plus=g)
+                gx = _mul_act_grad(gx, x, slope_in, out=gx, plus=g)
         return (gx, g if need[1] else None, gw1 if need[2] else None, gb1 if need[3] else None,
                 gw2 if need[4] else None, gb2 if need[5] else None,
-                None, None, None, None, None, None, None, None, None, None, None)
+                None, None, None, None, None, None, None, None, None, None, None, None)
 
 
 def res_block(x, plus, conv1, conv2, slope_in, slope_mid, slope_out):
@@ -173,21 +235,26 @@ def res_block(x, plus, conv1, conv2, slope_in, slope_mid, slope_out):
     pf2, pd2 = conv2._train_precisions()
     return _ResBlock.apply(x, plus, conv1.weight, conv1.bias, conv2.weight, conv2.bias, slope_in, slope_mid, slope_out,
                            conv1.packed_weight(pf1), conv2.packed_weight(pf2), conv1.dgrad_weight(pd1),
-                           conv2.dgrad_weight(pd2), pf1, pd1, pf2, pd2)
+                           conv2.dgrad_weight(pd2), pf1, pd1, pf2, pd2, conv1.act_storage)
 
 
 class _AddScaled(torch.autograd.Function):
     """a + b * scale[n, c] (+ c2)."""
 
     @staticmethod
-    def forward(ctx, a, b, scale, c2):
-        ctx.save_for_backward(b if scale is not None else None, scale)
+    def forward(ctx, a, b, scale, c2, storage):
+        ctx.kept = None
+        if scale is not None and storage is not None:
+            ctx.kept, tensors = _keep((b,), None, storage, ctx.needs_input_grad[2])
+            ctx.save_for_backward(scale, *tensors)
+        else:
+            ctx.save_for_backward(scale, b if scale is not None else None)
         ctx.has_c2 = c2 is not None
         return ops.add_scaled(a, b, scale, c2)
 
     @staticmethod
     def backward(ctx, g):
-        b, scale = ctx.saved_tensors
+        scale, *b = ctx.saved_tensors
         g = _rows_ok(g)
         need = ctx.needs_input_grad
         gb = gs = None
@@ -197,12 +264,13 @@ class _AddScaled(torch.autograd.Function):
             if need[1]:
                 gb = ops.scale_planes(g, scale)
             if need[2]:
+                b = b[0] if ctx.kept is None else ops.act_restore(_kept(ctx.kept, b)[0])
                 gs = ops.plane_dot(g, b).view_as(scale)
-        return (g if need[0] else None, gb, gs, g if (ctx.has_c2 and need[3]) else None)
+        return (g if need[0] else None, gb, gs, g if (ctx.has_c2 and need[3]) else None, None)
 
 
-def add_scaled(a, b, scale=None, c2=None):
-    return _AddScaled.apply(a, b, scale, c2)
+def add_scaled(a, b, scale=None, c2=None, storage=None):
+    return _AddScaled.apply(a, b, scale, c2, storage)
 
 
 class _FlowWarp(torch.autograd.Function):
@@ -273,29 +341,31 @@ def bilinear_up2(x, scale=1.0):
 class _SEGate(torch.autograd.Function):
     """gate[n, c] = sigmoid(fc2 relu(fc1 mean_hw(x)))  (reference layers.py:267-280).  The plane
     means run on the HIP reduction kernels; the adjoint of the two tiny FC layers (C x C/16
-    matrices on an (N, C) vector) is evaluated with torch on those few numbers."""
+    matrices on an (N, C) vector) is evaluated with torch on those few numbers.  With 8-bit storage the means are
+    taken in the forward pass and x itself is not kept."""
 
     @staticmethod
-    def forward(ctx, x, fc1, fc2):
-        ctx.save_for_backward(x, fc1, fc2)
+    def forward(ctx, x, fc1, fc2, storage):
+        ctx.shape, ctx.means = x.shape, storage is not None
+        ctx.save_for_backward(ops.plane_dot(x) if ctx.means else x, fc1, fc2)
         return ops.se_gate(x, fc1, fc2)
 
     @staticmethod
     def backward(ctx, g):
         x, fc1, fc2 = ctx.saved_tensors
-        n, c, h, w = x.shape
-        mean = (ops.plane_dot(x) / float(h * w)).view(n, c)
+        n, c, h, w = ctx.shape
+        mean = ((x if ctx.means else ops.plane_dot(x)) / float(h * w)).view(n, c)
         with torch.enable_grad():
             m = mean.detach().requires_grad_()
             a, b = fc1.detach().requires_grad_(), fc2.detach().requires_grad_()
             gate = torch.sigmoid(torch.relu(m @ a.t()) @ b.t())
             gm, ga, gb = torch.autograd.grad(gate, (m, a, b), g.reshape(n, c))
         gx = (gm / float(h * w)).view(n, c, 1, 1).expand(n, c, h, w) if ctx.needs_input_grad[0] else None
-        return gx, ga, gb
+        return gx, ga, gb, None
 
 
-def se_gate(x, fc1, fc2):
-    return _SEGate.apply(x, fc1, fc2)
+def se_gate(x, fc1, fc2, storage=None):
+    return _SEGate.apply(x, fc1, fc2, storage)
 
 
 class _RoundSTE(torch.autograd.Function):
@@ -410,3 +480,29 @@ class _SqErrSum(torch.autograd.Function):
 
 def sq_err_sum(a, b):
     return _SqErrSum.apply(a, b)
+
+
+class _SymbolLogProbs(torch.autograd.Function):
+    """-> (log_prob, entropy, top_log_prob | None, top_symbol | None) of ops.symbol_log_probs; the first two are
+    differentiable with respect to the logits, the alternatives are not."""
+
+    @staticmethod
+    def forward(ctx, logits, symbols, top):
+        r = ops.symbol_log_probs(logits, symbols, top)
+        ctx.save_for_backward(logits, symbols, r.stats, r.entropy)
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(r.top_log_prob, r.top_symbol)
+        return r.log_prob, r.entropy, r.top_log_prob, r.top_symbol
+
+    @staticmethod
+    def backward(ctx, g_lp, g_h, _top_lp, _top_sym):
+        if g_lp is None and g_h is None:
+            return None, None, None
+        logits, symbols, stats, entropy = ctx.saved_tensors
+        return ops.symbol_log_probs_backward(logits, symbols, stats, entropy, None if g_lp is None else g_lp.contiguous(),
+                                             None if g_h is None else g_h.contiguous()), None, None
+
+
+def symbol_log_probs(logits, symbols, top=0):
+    return _SymbolLogProbs.apply(logits, symbols, top)

@@ -1,0 +1,164 @@
+// Weight gradient of the 2-D convolutions from 8-bit activation checkpoints: entry points, plan and the reduction of the
+// partial results (the kernels are in conv_wgrad_ckpt_impl.h).
+#include "conv_wgrad_ckpt_impl.h"
+
+namespace dvc_wgrad_ckpt {
+
+int launch_aligned(int ks, int stride, const Args& a, const Plan& p, hipStream_t st) { return launch_shape<true>(ks, stride, a, p, st); }
+
+namespace {
+
+// gW[co][ci][tap] = sum over splits of partial[split][tap][co][ci], gB[co] likewise (indices past the weight's).  A block
+// takes 64 results; each of its waves adds every fourth split, the four sums are added in a fixed order.
+__global__ __launch_bounds__(256) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int nsplit, int taps, int cout, int cin,
+                                                                int cout_pad, int cin_pad, const float* bias_partial, float* gb) {
+  __shared__ float part[4][64];
+  const long long total = (long long)cout * taps * cin;
+  const long long total_all = total + (gb != nullptr ? cout : 0);
+  const int lane = threadIdx.x & 63, kg = threadIdx.x >> 6;
+  for (long long i0 = blockIdx.x * 64LL; i0 < total_all; i0 += (long long)gridDim.x * 64) {
+    const long long i = i0 + lane;
+    const float* p = nullptr;
+    long long step = 0, dst = -1;
+    if (i < total) {
+      const int ci = (int)(i % cin);
+      const long long q = i / cin;
+      const int tap = (int)(q % taps), co = (int)(q / taps);
+      p = partial + ((long long)tap * cout_pad + co) * cin_pad + ci;
+      step = (long long)taps * cout_pad * cin_pad;
+      dst = ((long long)co * cin + ci) * taps + tap;
+    } else if (i < total_all) {
+      p = bias_partial + (i - total);
+      step = cout_pad;
+    }
+    float s = 0.f;
+    if (p != nullptr)
+      for (int k = kg; k < nsplit; k += 4) s += p[k * step];
+    part[kg][lane] = s;
+    __syncthreads();
+    if (kg == 0 && p != nullptr) {
+      const float v = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+      if (dst >= 0) gw[dst] = v;
+      else gb[i - total] = v;
+    }
+    __syncthreads();
+  }
+}
+
+int make_plan(int cout, int cin, int ks, int stride, int batch, int h, int w, Plan* p, const char* who) {
+  DVC_REQUIRE(ks == 1 || ks == 3 || ks == 7, "%s: ksize=%d unsupported", who, ks);
+  DVC_REQUIRE(stride == 1 || stride == 2, "%s: stride=%d unsupported", who, stride);
+  DVC_REQUIRE(!(ks == 7 && stride != 1), "%s: 7x7 stride 2 unsupported", who);
+  DVC_REQUIRE(cout >= 1 && cin >= 1 && batch >= 1 && h >= 1 && w >= 1, "%s: bad dims", who);
+  DVC_REQUIRE((long long)h * w < (1LL << 28), "%s: plane too large", who);
+  const int pad = ks / 2;
+  p->ho = (h + 2 * pad - ks) / stride + 1;
+  p->wo = (w + 2 * pad - ks) / stride + 1;
+  // layers that fill a 32 x 32 block badly and whose fp32 form is narrower: 7x7 with a handful of channels
+  p->restore = ks == 7 && (cout <= 4 || cin <= 8);
+  p->tw = ks == 3 && stride == 1 && p->wo <= 16 ? 16 : 32;
+  p->mt = (cout > 32 && ks != 7) ? 2 : 1;
+  p->ct = (cin > 32 && ks != 7) ? 2 : 1;
+  p->th = ks == 1 ? 4 : (stride == 2 && p->mt * p->ct > 1 ? 2 : 4) * (32 / p->tw);
+  p->tiles_x = (p->wo + p->tw - 1) / p->tw;
+  p->tiles_y = (p->ho + p->th - 1) / p->th;
+  const long long nt = (long long)batch * p->tiles_x * p->tiles_y;
+  DVC_REQUIRE(nt < (1LL << 29), "%s: too many tiles", who);
+  p->n_tiles = (int)nt;
+  const int cob = 32 * p->mt, cib = 32 * p->ct;
+  p->cout_pad = (cout + cob - 1) / cob * cob;
+  p->cin_pad = (cin + cib - 1) / cib * cib;
+  p->n_cib = p->cin_pad / cib;
+  p->blocks = (p->cout_pad / cob) * p->n_cib;
+  p->taps = ks * ks;
+  // one 8-wave workgroup fits a CU: about one round of them
+  int s = (256 + p->blocks - 1) / p->blocks;
+  p->nsplit = s > p->n_tiles ? p->n_tiles : s;
+  return DVC_OK;
+}
+
+int check_srcs(const DvcCkpt* srcs, int n_src, int* cin, const char* who) {
+  DVC_REQUIRE(srcs != nullptr && n_src >= 1 && n_src <= DVC_MAX_SRC, "%s: n_src=%d not in 1..%d", who, n_src, DVC_MAX_SRC);
+  *cin = 0;
+  for (int s = 0; s < n_src; ++s) {
+    DVC_REQUIRE(srcs[s].codes != nullptr && srcs[s].scales != nullptr && srcs[s].channels >= 1, "%s: bad source %d", who, s);
+    DVC_REQUIRE(reinterpret_cast<uintptr_t>(srcs[s].codes) % 16 == 0, "%s: source %d: codes must start on 16 bytes", who, s);
+    DVC_REQUIRE(srcs[s].format == srcs[0].format && (srcs[s].format == DVC_CKPT_INT8 || srcs[s].format == DVC_CKPT_E4M3),
+                "%s: source %d: format %d", who, s, srcs[s].format);
+    *cin += srcs[s].channels;
+  }
+  return DVC_OK;
+}
+
+}  // namespace
+}  // namespace dvc_wgrad_ckpt
+
+using namespace dvc_wgrad_ckpt;
+
+extern "C" int64_t dvc_conv2d_wgrad_ckpt_scratch_floats(int32_t cout, int32_t cin, int32_t ksize, int32_t stride,
+                                                        int32_t batch, int32_t in_h, int32_t in_w) {
+  Plan p;
+  if (int rc = make_plan(cout, cin, ksize, stride, batch, in_h, in_w, &p, "dvc_conv2d_wgrad_ckpt_scratch_floats")) return rc;
+  if (p.restore) {
+    const int64_t n = dvc_conv2d_wgrad_scratch_floats(cout, cin, ksize, stride, batch, in_h, in_w);
+    return n < 0 ? n : n + (int64_t)batch * cin * in_h * in_w;
+  }
+  return (int64_t)p.nsplit * p.taps * p.cout_pad * p.cin_pad + (int64_t)p.nsplit * p.cout_pad;
+}
+
+extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t batch, int32_t in_h, int32_t in_w,
+                                     const float* grad_out, int32_t out_channels, int32_t ksize, int32_t stride,
+                                     float* scratch, float* grad_weight, float* grad_bias, void* stream) {
+  const char* const who = "dvc_conv2d_wgrad_ckpt";
+  int cin;
+  if (int rc = check_srcs(srcs, n_src, &cin, who)) return rc;
+  DVC_REQUIRE(grad_out != nullptr && scratch != nullptr && grad_weight != nullptr, "%s: null pointer", who);
+  Plan p;
+  if (int rc = make_plan(out_channels, cin, ksize, stride, batch, in_h, in_w, &p, who)) return rc;
+  if (p.restore) {
+    const int64_t plane = (int64_t)in_h * in_w;
+    const DvcSrc x{scratch, cin * plane, plane, cin, 0};
+    int c0 = 0;
+    for (int s = 0; s < n_src; ++s) {
+      const DvcDst d{scratch + c0 * plane, cin * plane, plane};
+      if (int rc = dvc_act_restore(&srcs[s], &d, batch, in_h, in_w, stream)) return rc;
+      c0 += srcs[s].channels;
+    }
+    return dvc_conv2d_wgrad(&x, 1, batch, in_h, in_w, 0, 1.f, grad_out, out_channels, ksize, stride, scratch + batch * cin * plane,
+                            grad_weight, grad_bias, stream);
+  }
+  Args a{};
+  int first = 0;
+  for (int s = 0; s < DVC_MAX_SRC; ++s) {
+    const bool have = s < n_src;
+    a.codes[s] = have ? srcs[s].codes : srcs[0].codes;
+    a.scales[s] = have ? srcs[s].scales : srcs[0].scales;
+    a.first[s] = have ? first : cin;
+    a.chans[s] = have ? srcs[s].channels : 1;
+    first += have ? srcs[s].channels : 0;
+  }
+  a.e4m3 = srcs[0].format == DVC_CKPT_E4M3;
+  a.cin = cin;
+  a.h = in_h;
+  a.w = in_w;
+  a.blocks = (int)(((long long)in_h * in_w + 31) / 32);
+  a.cout = out_channels;
+  a.ho = p.ho;
+  a.wo = p.wo;
+  a.g = grad_out;
+  a.partial = scratch;
+  a.bias_partial = grad_bias != nullptr ? scratch + (long long)p.nsplit * p.taps * p.cout_pad * p.cin_pad : nullptr;
+  a.cout_pad = p.cout_pad;
+  a.cin_pad = p.cin_pad;
+  a.n_cib = p.n_cib;
+  a.tiles_x = p.tiles_x;
+  a.tiles_y = p.tiles_y;
+  a.n_tiles = p.n_tiles;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool aligned = in_w % 4 == 0 && p.wo % 4 == 0 && reinterpret_cast<uintptr_t>(grad_out) % 16 == 0;
+  if (int rc = aligned ? launch_aligned(ksize, stride, a, p, st) : launch_any(ksize, stride, a, p, st)) return rc;
+  const long long total = (long long)out_channels * cin * p.taps + out_channels;
+  hipLaunchKernelGGL(wgrad_ckpt_reduce_kernel, dim3(dvc::stream_grid(total, 64)), dim3(256), 0, st, scratch, grad_weight, p.nsplit,
+                     p.taps, out_channels, cin, p.cout_pad, p.cin_pad, a.bias_partial, grad_bias);
+  return dvc::check_launch("wgrad_ckpt_reduce_kernel");
+}

@@ -1,0 +1,500 @@
+// Weight gradient of the 2-D convolutions from 8-bit activation checkpoints (include/dvc_hip.h): the kernels.
+//
+//   gW[co][ci][ky][kx] = sum over (n, oy, ox) of  g[n][co][oy][ox] * X[n][ci][oy*s + ky - p][ox*s + kx - p]
+//
+// Mathematics.  A checkpoint's value is (at most seven bits) * 2^e: exactly a bf16 number.  An fp32 gradient is exactly
+// the sum of three bf16 numbers of eight bits each (cut off, subtract, cut off, subtract).  So gW is three bf16
+// matrix products with exact products and fp32 sums -- the accuracy of the fp32 kernel at 2.5 PFLOP/s / 3 instead of 157
+// TFLOP/s: it is the 8-bit storage that buys the rate.
+//
+// Shape.  [Cout x pixels] * [pixels x Cin taps], a small result and a very long reduction, on
+// v_mfma_f32_32x32x16_bf16: rows = 32 output channels, columns = 32 input channels at one tap, k = 16 adjacent
+// pixels of a row (a half-wave holds 8 of them: one 16-byte LDS read).  The taps of a row read the same 16-byte windows,
+// shifted by whole elements in registers (v_alignbit): nine products of a 3x3 layer need three window reads.
+// A workgroup (8 waves) owns (32 MT) x (32 CT) of the result for all taps; the 8 / (MT CT) waves of one 32 x 32 corner
+// take the row pieces of a tile in turn and are added through LDS in a fixed order at the end.  The pixel axis is cut
+// into slabs whose partial results a second kernel adds in a fixed order (deterministic, no atomics).
+//
+// Staging per tile of TH x TW output pixels, two LDS buffers and one barrier per tile: while a tile is multiplied the next
+// one's codes, scales and gradients (loaded during the tile before) are decoded to bf16 / stored as fp32 into the other
+// buffer, and the loads of the one after are issued.  A lane decodes four codes of a row (one dword).  The gradient stays
+// fp32 in LDS (4 instead of 6 bytes) and is split when it is read; the bias gradient is summed by the lanes that stage it.
+// Channel strides in LDS are odd multiples of 16 bytes: 16 lanes of a read (16 channels) fall on all 64 banks.
+#pragma once
+#include <atomic>
+#include <type_traits>
+
+#include "dvc_common.h"
+
+namespace dvc_wgrad_ckpt {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+struct Args {
+  const uint8_t* codes[DVC_MAX_SRC];
+  const uint8_t* scales[DVC_MAX_SRC];
+  int first[DVC_MAX_SRC];       // first channel of each source; sources that are not there start at cin
+  int chans[DVC_MAX_SRC];
+  int e4m3;
+  int cin, h, w, blocks;        // blocks of 32 per plane
+  int cout, ho, wo;
+  const float* g;               // [N][cout][ho][wo], contiguous
+  float* partial;               // [S][taps][cout_pad][cin_pad]
+  float* bias_partial;          // [S][cout_pad], or null
+  int cout_pad, cin_pad, n_cib;
+  int tiles_x, tiles_y, n_tiles;
+};
+
+__device__ __forceinline__ unsigned long long uniform64(unsigned long long v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v);
+  const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+  return ((unsigned long long)hi << 32) | lo;
+}
+
+// Where input channel `ci` (uniform) of the concatenated checkpoints lives: its plane's blocks in sample 0 counted from the
+// source's first, and the blocks between samples.  Channels past the last: live = 0.
+struct Plane {
+  unsigned long long codes, scales;      // addresses of sample 0's plane
+  unsigned long long step;               // blocks between samples
+  unsigned live;                         // all-ones or zero
+};
+__device__ __forceinline__ Plane plane_of(const Args& a, int ci) {
+  // (mask arithmetic instead of indexing by a run-time source number, which would become a private lookup table)
+  const unsigned long long m1 = 0ull - (unsigned long long)(ci >= a.first[1]);
+  const unsigned long long m2 = 0ull - (unsigned long long)(ci >= a.first[2]);
+  const unsigned long long m3 = 0ull - (unsigned long long)(ci >= a.first[3]);
+  auto pick = [&](unsigned long long v0, unsigned long long v1, unsigned long long v2, unsigned long long v3) {
+    return v0 + ((v1 - v0) & m1) + ((v2 - v1) & m2) + ((v3 - v2) & m3);
+  };
+  const unsigned long long c = pick((unsigned long long)a.codes[0], (unsigned long long)a.codes[1], (unsigned long long)a.codes[2],
+                                    (unsigned long long)a.codes[3]);
+  const unsigned long long s = pick((unsigned long long)a.scales[0], (unsigned long long)a.scales[1],
+                                    (unsigned long long)a.scales[2], (unsigned long long)a.scales[3]);
+  const unsigned long long first = pick(a.first[0], a.first[1], a.first[2], a.first[3]);
+  const unsigned long long chans = pick(a.chans[0], a.chans[1], a.chans[2], a.chans[3]);
+  const bool have = ci < a.cin;
+  const unsigned long long at = have ? ((unsigned long long)ci - first) * (unsigned)a.blocks : 0ull;
+  Plane p;
+  p.codes = uniform64((have ? c : (unsigned long long)a.codes[0]) + 32ull * at);
+  p.scales = uniform64((have ? s : (unsigned long long)a.scales[0]) + at);
+  p.step = uniform64(have ? chans * (unsigned)a.blocks : 0ull);
+  p.live = __builtin_amdgcn_readfirstlane(have ? 0xffffffffu : 0u);
+  return p;
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(unsigned long long at, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(at), 0, bytes, 0x00020000);
+}
+
+struct __attribute__((packed)) Dword { unsigned v; };      // a dword at any byte address
+
+__device__ __forceinline__ float scale_of(unsigned s) { return s == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(s << 23); }
+
+// four codes -> two dwords of bf16 (exact); s01 / s23 ... one scale per code
+template <bool E4M3>
+__device__ __forceinline__ uint2 decode(unsigned k, float s0, float s1, float s2, float s3) {
+  uint2 r;
+  if constexpr (E4M3) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)k, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)k, true);
+    r.x = __builtin_amdgcn_perm(__float_as_uint(lo[1] * s1), __float_as_uint(lo[0] * s0), 0x07060302u);
+    r.y = __builtin_amdgcn_perm(__float_as_uint(hi[1] * s3), __float_as_uint(hi[0] * s2), 0x07060302u);
+  } else {
+    const unsigned m = k & 0x7f7f7f7fu, sg = k & 0x80808080u;
+    const float f0 = (float)(m & 0xffu) * s0, f1 = (float)((m >> 8) & 0xffu) * s1;
+    const float f2 = (float)((m >> 16) & 0xffu) * s2, f3 = (float)(m >> 24) * s3;
+    r.x = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u) | __builtin_amdgcn_perm(0u, sg, 0x010c000cu);
+    r.y = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u) | __builtin_amdgcn_perm(0u, sg, 0x030c020cu);
+  }
+  return r;
+}
+
+// eight gradients -> three fragments of bf16 that add up to them
+struct Split { bf16x8 a1, a2, a3; };
+__device__ __forceinline__ Split split(const float4 lo, const float4 hi) {
+  const float g[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  u32x4 p1, p2, p3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned b1[2], b2[2], b3[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float v = g[2 * i + j];
+      b1[j] = __float_as_uint(v);
+      const float r = v - __uint_as_float(b1[j] & 0xffff0000u);
+      b2[j] = __float_as_uint(r);
+      b3[j] = __float_as_uint(r - __uint_as_float(b2[j] & 0xffff0000u));
+    }
+    p1[i] = __builtin_amdgcn_perm(b1[1], b1[0], 0x07060302u);
+    p2[i] = __builtin_amdgcn_perm(b2[1], b2[0], 0x07060302u);
+    p3[i] = __builtin_amdgcn_perm(b3[1], b3[0], 0x07060302u);
+  }
+  return Split{__builtin_bit_cast(bf16x8, p1), __builtin_bit_cast(bf16x8, p2), __builtin_bit_cast(bf16x8, p3)};
+}
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// eight elements from element `e` on of the dwords d[] (two elements each)
+template <int E, int D>
+__device__ __forceinline__ bf16x8 window(const unsigned (&d)[D]) {
+  static_assert(E / 2 + (E % 2 ? 5 : 4) <= D, "window past the dwords read");
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = E % 2 ? __builtin_amdgcn_alignbit(d[E / 2 + i + 1], d[E / 2 + i], 16) : d[E / 2 + i];
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// Geometry.  KS x KS taps, stride S, tiles of TH x TW output pixels; a staged input row is XD dwords of codes from column
+// gx0 = ox0 * S - LEFT on (a multiple of 4), kept in LDS as XROW bf16: as it is (stride 1), or its even columns, then
+// (3x3) its odd ones, so that the eight pixels of a half-wave are adjacent at stride 2 as well.
+template <int KS, int S, int MT, int CT, int TW_>
+struct Geo {
+  static constexpr int KG = KS == 7 ? 1 : 8 / (MT * CT);         // waves sharing one corner (7x7: one tap row per wave)
+  static constexpr int XCH = 32 * CT, GCH = 32 * MT;
+  static constexpr int TAPS = KS * KS, ACC = KS == 7 ? 7 : TAPS; // accumulator tiles per wave
+  static_assert(KS != 7 || (S == 1 && MT == 1 && CT == 1), "7x7: 32 x 32 blocks, stride 1");
+  static constexpr int TW = TW_, TH = KS == 1 ? 4 : (S == 2 && KG < 8 ? 2 : 4) * (32 / TW_), PAD = KS / 2;
+  static constexpr int LEFT = KS == 1 ? 0 : 4;
+  static constexpr int YS = KS == 1 ? S : 1;                     // input rows between staged rows
+  static constexpr int IH = KS == 1 ? TH : (TH - 1) * S + KS;
+  static constexpr int XD = (TW * S + (KS == 1 ? 0 : 8)) / 4;    // dwords (4 codes) per staged row
+  static constexpr int ODD = TW + 8;                             // odd columns of a stride-2 row
+  static constexpr int XROW = S == 1 ? 4 * XD : KS == 1 ? TW : TW + ODD;
+  static_assert(XROW % 8 == 0, "rows on 16 bytes");
+  static constexpr int XUNITS = (IH * XROW / 8) | 1;             // 16-byte units per channel, odd
+  static constexpr int GUNITS = (TH * TW / 4) | 1;
+  static constexpr int XE = IH * XD, XSLOTS = (XE + 63) / 64;
+  static constexpr int XPW = XCH / 8;                            // channels of x staged per wave
+  static constexpr int GE = TH * TW / 4, GLOADS = GCH * GE / 512;
+  static_assert(GCH * GE % 512 == 0, "gradient units deal out evenly");
+  static constexpr int XBYTES = XCH * XUNITS * 16, BUF = XBYTES + GCH * GUNITS * 16;
+  static constexpr int RED = (KG - 1) * MT * CT * 4096;
+  static constexpr int LDS_BYTES = 2 * BUF > RED ? 2 * BUF : RED;
+  static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+  static constexpr int STEPS = TH * TW / 16;                     // row pieces of 16 pixels per tile
+  static_assert(STEPS % KG == 0, "row pieces deal out evenly");
+};
+
+// AL: rows of codes start on dwords and rows of gradients on 16 bytes (w % 4 == 0, wo % 4 == 0).
+template <int KS, int S, int MT, int CT, int TW, bool AL>
+__global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
+  using G = Geo<KS, S, MT, CT, TW>;
+  constexpr int KG = G::KG, XPW = G::XPW, XSLOTS = G::XSLOTS, GLOADS = G::GLOADS, TAPS = G::TAPS, ACC = G::ACC;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int corner = KS == 7 ? 0 : wave % (MT * CT), grp = KS == 7 ? 0 : wave / (MT * CT);
+  const int mt = corner / CT, ct = corner % CT;
+  const int cob = blockIdx.y / a.n_cib, cib = blockIdx.y - cob * a.n_cib;
+  const int co0 = cob * G::GCH, ci0 = cib * G::XCH;
+  const int nsplit = gridDim.x;
+  const int per_n = a.tiles_x * a.tiles_y;
+  const unsigned plane_bytes = 32u * (unsigned)a.blocks;
+  const unsigned gplane = (unsigned)(a.ho * a.wo);
+
+  Plane xp[XPW];
+#pragma unroll
+  for (int c = 0; c < XPW; ++c) xp[c] = plane_of(a, ci0 + XPW * wave + c);
+  // gradient units: unit u = tid + 512 i is unit u % GE of channel u / GE
+  unsigned gsrc[GLOADS];        // this lane's channel, as an offset in planes; past the last channel: none
+  int gdst[GLOADS];
+#pragma unroll
+  for (int i = 0; i < GLOADS; ++i) {
+    const int u = tid + 512 * i, ch = u / G::GE, e = u - ch * G::GE;
+    gsrc[i] = co0 + ch < a.cout ? (unsigned)(co0 + ch) : 0xffffffffu;
+    gdst[i] = G::XBYTES + (ch * G::GUNITS + e) * 16;
+  }
+  float gsum[GLOADS];
+#pragma unroll
+  for (int i = 0; i < GLOADS; ++i) gsum[i] = 0.f;
+
+  unsigned xk[XPW][XSLOTS], xs[XPW][XSLOTS], xs2[AL ? 1 : XPW][AL ? 1 : XSLOTS];
+  int mask[XSLOTS];             // codes of a dword inside the row (not AL)
+  int cut[XSLOTS];              // codes of a dword before a block's end (not AL)
+  float4 gr[GLOADS];
+
+  auto load = [&](int t) {      // request tile t (past the last: zeros)
+    const bool there = t < a.n_tiles;
+    const int tt = there ? t : 0;
+    const int n = tt / per_n, r = tt - n * per_n;
+    const int ty = r / a.tiles_x, tx = r - ty * a.tiles_x;
+    const int oy0 = ty * G::TH, ox0 = tx * TW;
+    const int gy0 = KS == 1 ? oy0 * S : oy0 * S - G::PAD, gx0 = ox0 * S - G::LEFT;
+    unsigned off[XSLOTS];
+#pragma unroll
+    for (int j = 0; j < XSLOTS; ++j) {
+      const int e = lane + 64 * j, iy = e / G::XD, q = e - iy * G::XD;
+      const int gy = gy0 + iy * G::YS, gx = gx0 + 4 * q;
+      const bool ok = e < G::XE && gy >= 0 && gy < a.h && gx >= 0 && gx < a.w;
+      off[j] = ok ? (unsigned)(gy * a.w + gx) : 0x80000000u;
+      if constexpr (!AL) {
+        mask[j] = ok ? (a.w - gx < 4 ? a.w - gx : 4) : 0;
+        cut[j] = 32 - (int)(off[j] & 31u);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < XPW; ++c) {
+      const unsigned long long b = (unsigned long long)(unsigned)n * xp[c].step;
+      const unsigned live = there ? xp[c].live : 0u;
+#pragma unroll
+      for (int j = 0; j < XSLOTS; ++j) {
+        if constexpr (AL) {
+          xk[c][j] = __builtin_amdgcn_raw_buffer_load_b32(rsrc(xp[c].codes + 32ull * b, plane_bytes & live), off[j], 0, 0);
+          xs[c][j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(xp[c].scales + b, (unsigned)a.blocks & live), off[j] >> 5, 0, 0);
+        } else {
+          // the dword may reach past the plane's last byte: read the last four and shift
+          const bool ok = mask[j] > 0 && live;
+          const unsigned at = ok ? off[j] : 0u;
+          const unsigned from = at < plane_bytes - 4u ? at : plane_bytes - 4u;
+          const unsigned k = reinterpret_cast<const Dword*>(xp[c].codes + 32ull * b + from)->v >> (8u * (at - from));
+          xk[c][j] = ok ? k : 0u;
+          const uint8_t* const sp = reinterpret_cast<const uint8_t*>(xp[c].scales + b);
+          const unsigned last = (unsigned)a.blocks - 1u, b2 = (at + 3u) >> 5;
+          xs[c][j] = sp[at >> 5];
+          xs2[c][j] = sp[b2 < last ? b2 : last];
+        }
+      }
+    }
+    // gradients: four adjacent pixels of a row
+#pragma unroll
+    for (int i = 0; i < GLOADS; ++i) {
+      const int u = tid + 512 * i, e = u % G::GE;
+      const int oy = oy0 + 4 * e / TW, ox = ox0 + 4 * e % TW;
+      const bool ok = there && gsrc[i] != 0xffffffffu && oy < a.ho && ox < a.wo;
+      const float* const p = a.g + ((unsigned long long)(unsigned)n * a.cout + (ok ? gsrc[i] : 0u)) * gplane + (ok ? oy * a.wo + ox : 0);
+      gr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ok) {
+        if constexpr (AL) {
+          gr[i] = *reinterpret_cast<const float4*>(p);
+        } else {
+          gr[i].x = p[0];
+          if (ox + 1 < a.wo) gr[i].y = p[1];
+          if (ox + 2 < a.wo) gr[i].z = p[2];
+          if (ox + 3 < a.wo) gr[i].w = p[3];
+        }
+      }
+    }
+  };
+
+  auto store_as = [&](char* buf, auto e4m3) {      // decode what load() requested into an LDS buffer
+#pragma unroll
+    for (int j = 0; j < XSLOTS; ++j) {
+      const int e = lane + 64 * j, iy = e / G::XD, q = e - iy * G::XD;
+#pragma unroll
+      for (int c = 0; c < XPW; ++c) {
+        const float s0 = scale_of(xs[c][j]);
+        uint2 v;
+        if constexpr (AL) {
+          v = decode<decltype(e4m3)::value>(xk[c][j], s0, s0, s0, s0);
+        } else {
+          const float s4 = scale_of(xs2[c][j]);
+          v = decode<decltype(e4m3)::value>(xk[c][j], s0, cut[j] > 1 ? s0 : s4, cut[j] > 2 ? s0 : s4, cut[j] > 3 ? s0 : s4);
+          // codes past the row's end are padding: zeros (also where the scale is that of a poisoned block)
+          v.x = mask[j] > 1 ? v.x : mask[j] > 0 ? v.x & 0xffffu : 0u;
+          v.y = mask[j] > 3 ? v.y : mask[j] > 2 ? v.y & 0xffffu : 0u;
+        }
+        if (64 * (j + 1) <= G::XE || e < G::XE) {
+          char* const row = buf + ((XPW * wave + c) * G::XUNITS * 8 + iy * G::XROW) * 2;
+          if constexpr (S == 1) {
+            *reinterpret_cast<uint2*>(row + 8 * q) = v;
+          } else {
+            const unsigned even = __builtin_amdgcn_perm(v.y, v.x, 0x05040100u), odd = __builtin_amdgcn_perm(v.y, v.x, 0x07060302u);
+            if constexpr (KS == 1) {
+              *reinterpret_cast<unsigned*>(row + 4 * q) = even;
+            } else {
+              // even columns from column 4 on (the middle tap's), odd ones from column 1 on
+              if (q >= 1 && q <= TW / 2) *reinterpret_cast<unsigned*>(row + 4 * (q - 1)) = even;
+              *reinterpret_cast<unsigned*>(row + 2 * TW + 4 * q) = odd;
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < GLOADS; ++i) {
+      *reinterpret_cast<float4*>(buf + gdst[i]) = gr[i];
+      gsum[i] += (gr[i].x + gr[i].y) + (gr[i].z + gr[i].w);
+    }
+  };
+
+  auto store = [&](char* buf) {
+    if (a.e4m3) store_as(buf, std::true_type{});
+    else store_as(buf, std::false_type{});
+  };
+
+  f32x16 acc[ACC];
+#pragma unroll
+  for (int t = 0; t < ACC; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+
+  const int ga = G::XBYTES + (mt * 32 + l32) * G::GUNITS * 16 + half * 32;
+  const int xa = (ct * 32 + l32) * G::XUNITS * 16 + half * 16;
+
+  auto multiply = [&](const char* buf, int step) {       // one row piece
+    const int row = step / (TW / 16), px = step % (TW / 16) * 16;
+    const float4* const gp = reinterpret_cast<const float4*>(buf + ga + (row * TW + px) * 4);
+    const Split s = split(gp[0], gp[1]);
+    constexpr int ROWS = KS == 7 ? 1 : KS;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int ky = KS == 7 ? wave : i;
+      const char* const xr = buf + xa + ((KS == 1 ? row : row * S + ky) * G::XROW + px) * 2;
+      bf16x8 b[KS];
+      if constexpr (KS == 1) {
+        b[0] = *reinterpret_cast<const bf16x8*>(xr);
+      } else if constexpr (S == 1) {
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(xr), hi = *reinterpret_cast<const u32x4*>(xr + 16);
+        const unsigned d[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        if constexpr (KS == 3) {      // staged column 4 is pixel 0
+          b[0] = window<3>(d); b[1] = window<4>(d); b[2] = window<5>(d);
+        } else {
+          b[0] = window<1>(d); b[1] = window<2>(d); b[2] = window<3>(d); b[3] = window<4>(d);
+          b[4] = window<5>(d); b[5] = window<6>(d); b[6] = window<7>(d);
+        }
+      } else {
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(xr + 2 * TW);
+        const unsigned d[5] = {lo[0], lo[1], lo[2], lo[3], *reinterpret_cast<const unsigned*>(xr + 2 * TW + 16)};
+        b[0] = window<1>(d); b[2] = window<2>(d);
+        b[1] = *reinterpret_cast<const bf16x8*>(xr);
+      }
+#pragma unroll
+      for (int kx = 0; kx < KS; ++kx) acc[i * KS + kx] = mfma(s.a3, b[kx], acc[i * KS + kx]);
+#pragma unroll
+      for (int kx = 0; kx < KS; ++kx) acc[i * KS + kx] = mfma(s.a2, b[kx], acc[i * KS + kx]);
+#pragma unroll
+      for (int kx = 0; kx < KS; ++kx) acc[i * KS + kx] = mfma(s.a1, b[kx], acc[i * KS + kx]);
+    }
+  };
+
+  int t = blockIdx.x, b = 0;
+  load(t);
+  store(lds);
+  load(t + nsplit);
+  __syncthreads();
+  for (; t < a.n_tiles; t += nsplit) {
+    store(lds + (b ^ 1) * G::BUF);          // tile t + nsplit (zeros past the last)
+    load(t + 2 * nsplit);
+    const char* const buf = lds + b * G::BUF;
+    if (KS != 7 || wave < 7) {
+#pragma unroll
+      for (int i = 0; i < G::STEPS / KG; ++i) multiply(buf, i * KG + grp);
+    }
+    __syncthreads();
+    b ^= 1;
+  }
+
+  // bias gradient: the lanes of a channel are GE adjacent ones (a multiple of 32): butterfly within 32, then one atomic-free
+  // add per half through LDS below
+  float* const bs = reinterpret_cast<float*>(lds);      // [GCH][GE / 32]
+  if (a.bias_partial != nullptr && cib == 0) {
+    constexpr int SEG = G::GE < 64 ? G::GE : 64;         // adjacent lanes of one channel
+    static_assert(SEG == 16 || SEG == 32 || SEG == 64, "butterfly");
+#pragma unroll
+    for (int i = 0; i < GLOADS; ++i) {
+      float v = gsum[i];
+#pragma unroll
+      for (int m = SEG / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+      if ((lane & (SEG - 1)) == 0) bs[(tid + 512 * i) / SEG] = v;
+    }
+    __syncthreads();
+    constexpr int PARTS = G::GE / SEG;
+    if (tid < G::GCH) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) v += bs[tid * PARTS + k];
+      a.bias_partial[(long long)blockIdx.x * a.cout_pad + co0 + tid] = v;
+    }
+    __syncthreads();
+  }
+
+  // add the waves of a corner, tap by tap; register r of a tile is row (r & 3) + 8 (r >> 2) + 4 half, column l32
+  float* const red = reinterpret_cast<float*>(lds);
+  float* const pbase = a.partial + (long long)blockIdx.x * TAPS * a.cout_pad * a.cin_pad;
+  if constexpr (KS == 7) {
+    if (wave < 7) {
+#pragma unroll
+      for (int kx = 0; kx < 7; ++kx) {
+        float* const pt = pbase + (long long)(wave * 7 + kx) * a.cout_pad * a.cin_pad + ci0 + l32;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) pt[(long long)(co0 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = acc[kx][r];
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int tp = 0; tp < ACC; ++tp) {
+    if (KG > 1 && grp > 0) {
+      float* const dst = red + ((grp - 1) * (MT * CT) + corner) * 1024 + lane;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dst[64 * r] = acc[tp][r];
+    }
+    if (KG > 1) __syncthreads();
+    if (grp == 0) {
+      f32x16 v = acc[tp];
+#pragma unroll
+      for (int k = 1; k < KG; ++k) {
+        const float* const src = red + ((k - 1) * (MT * CT) + corner) * 1024 + lane;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] += src[64 * r];
+      }
+      float* const pt = pbase + (long long)tp * a.cout_pad * a.cin_pad + ci0 + ct * 32 + l32;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) pt[(long long)(co0 + mt * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = v[r];
+    }
+    if (KG > 1) __syncthreads();
+  }
+}
+
+struct Plan {
+  int ho, wo, tw, th, tiles_x, tiles_y, n_tiles, cout_pad, cin_pad, n_cib, blocks, nsplit, taps, mt, ct;
+  bool restore;      // no kernel for this shape here: restore and run the fp32 one
+};
+
+template <class K>
+int allow_lds(K kernel, int bytes, std::atomic<unsigned long long>* done, const char* what) {
+  // LDS above the default needs an opt-in per kernel and device (twice is harmless)
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device > 63) device = 0;
+  const unsigned long long bit = 1ull << device;
+  if (done->load(std::memory_order_acquire) & bit) return DVC_OK;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    dvc::set_error("hipFuncSetAttribute(%s): %s", what, hipGetErrorString(e));
+    return DVC_EHIP;
+  }
+  done->fetch_or(bit, std::memory_order_release);
+  return DVC_OK;
+}
+
+template <int KS, int S, int MT, int CT, int TW, bool AL>
+int launch(const Args& a, const Plan& p, hipStream_t st) {
+  using G = Geo<KS, S, MT, CT, TW>;
+  static std::atomic<unsigned long long> done{0};
+  if (int rc = allow_lds(&wgrad_ckpt_kernel<KS, S, MT, CT, TW, AL>, G::LDS_BYTES, &done, "wgrad_ckpt_kernel")) return rc;
+  hipLaunchKernelGGL((wgrad_ckpt_kernel<KS, S, MT, CT, TW, AL>), dim3(p.nsplit, p.blocks), dim3(512), G::LDS_BYTES, st, a);
+  return dvc::check_launch("wgrad_ckpt_kernel");
+}
+
+template <int KS, int S, int TW, bool AL>
+int launch_block(const Args& a, const Plan& p, hipStream_t st) {
+  if (p.mt == 2) return p.ct == 2 ? launch<KS, S, 2, 2, TW, AL>(a, p, st) : launch<KS, S, 2, 1, TW, AL>(a, p, st);
+  return p.ct == 2 ? launch<KS, S, 1, 2, TW, AL>(a, p, st) : launch<KS, S, 1, 1, TW, AL>(a, p, st);
+}
+
+template <bool AL>
+int launch_shape(int ks, int stride, const Args& a, const Plan& p, hipStream_t st) {
+  if (ks == 3 && stride == 1) return p.tw == 16 ? launch_block<3, 1, 16, AL>(a, p, st) : launch_block<3, 1, 32, AL>(a, p, st);
+  if (ks == 3) return launch_block<3, 2, 32, AL>(a, p, st);
+  if (ks == 7) return launch<7, 1, 1, 1, 32, AL>(a, p, st);
+  return stride == 1 ? launch_block<1, 1, 32, AL>(a, p, st) : launch_block<1, 2, 32, AL>(a, p, st);
+}
+
+int launch_aligned(int ks, int stride, const Args& a, const Plan& p, hipStream_t st);
+int launch_any(int ks, int stride, const Args& a, const Plan& p, hipStream_t st);
+
+}  // namespace dvc_wgrad_ckpt

@@ -1,0 +1,680 @@
+// Log probabilities of given symbols under distributions given class by class, with entropy, the most likely
+// alternatives, and the gradient (include/dvc_hip.h).
+//
+// Mathematics.  One pass over the logits l_v of a site with the running maximum m:
+//   S = sum e^(l_v - m),  T = sum e^(l_v - m) (l_v - m)   (both rescaled when m grows)
+//   log p_v = (l_v - m) - log S,   H = log S - T / S
+// S >= 1 and T <= 0, so both terms of H are >= 0 and nothing cancels.  m and log S are kept apart for the backward pass:
+// their sum would round away what distinguishes probabilities once |m| is large.
+//   dL/dl_v = g_lp (1[v = s] - p_v) - g_H p_v (log p_v + H)
+// Classes at minus infinity add nothing (0 * -inf is kept out by a floor on l_v - m in T); a NaN or +inf makes the whole
+// site NaN.  Everything is held in fp32 whatever the logits' type.
+#include "dvc_common.h"
+
+namespace {
+
+struct Logits { const void* p; long long bs, cs; int groups, classes; };
+
+template <int DT> struct Elem;
+template <> struct Elem<DVC_F32> {
+  typedef float type;
+  static __device__ __forceinline__ float up(float v) { return v; }
+  static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <> struct Elem<DVC_BF16> {
+  typedef unsigned short type;
+  static __device__ __forceinline__ float up(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
+  static __device__ __forceinline__ unsigned short down(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
+};
+template <> struct Elem<DVC_F16> {
+  typedef _Float16 type;
+  static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
+};
+
+// below this e^x is zero in fp32: a floor that keeps 0 * (-inf) out of the entropy sums
+constexpr float kFloor = -200.f;
+#define NEG_INF (-__builtin_inff())
+
+// the running statistics of one site (or of a part of its classes)
+struct Stat {
+  float m, s, t;
+  __device__ __forceinline__ void clear() { m = NEG_INF; s = 0.f; t = 0.f; }
+  // join with another part: either may be empty (m = -inf, s = 0)
+  __device__ __forceinline__ void join(float m2, float s2, float t2) {
+    const float mm = fmaxf(m, m2);
+    const float a = m == mm ? 1.f : __expf(m - mm), b = m2 == mm ? 1.f : __expf(m2 - mm);
+    t = a * (t + s * fmaxf(m == mm ? 0.f : m - mm, kFloor)) + b * (t2 + s2 * fmaxf(m2 == mm ? 0.f : m2 - mm, kFloor));
+    s = a * s + b * s2;
+    m = mm;
+  }
+  __device__ __forceinline__ void add(float x) {
+    if (x > m) {
+      const float a = __expf(m - x);
+      t = a * (t + s * fmaxf(m - x, kFloor));
+      s = a * s;
+      m = x;
+    }
+    const float d = m == NEG_INF ? x : x - m;   // (all classes so far at -inf: e = exp(-inf) = 0)
+    const float e = __expf(d);
+    s += e;
+    t += e * fmaxf(d, kFloor);
+  }
+};
+
+__device__ __forceinline__ void finish(const Stat& st, float* log_s, float* entropy) {
+  const bool empty = st.m == NEG_INF && st.s == 0.f;   // (s is NaN when a class was)
+  *log_s = empty ? 0.f : __logf(st.s);
+  *entropy = empty ? 0.f : *log_s - st.t / st.s;
+}
+
+// log p of a logit
+__device__ __forceinline__ float log_p(float x, float m, float log_s) {
+  return (x - (m == NEG_INF ? 0.f : m)) - log_s;
+}
+
+// log of the probability of the given symbol (bounds are checked here: nothing outside the row is read)
+template <int DT>
+__device__ __forceinline__ float given(const typename Elem<DT>::type* row, long long cs, int classes, int sym, float m, float log_s) {
+  if (sym < 0) return 0.f;
+  if (sym >= classes) return __uint_as_float(0x7fc00000u);
+  return log_p(Elem<DT>::up(row[sym * cs]), m, log_s);
+}
+
+// order of the alternatives: larger logit first, NaN above all, then the lower class.  +0 and -0 are equal.
+__device__ __forceinline__ unsigned order_key(float x) {
+  const unsigned b = __float_as_uint(x + 0.f);
+  return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+// ---------------------------------------------------------------- wave helpers
+__device__ __forceinline__ unsigned wave_max(unsigned v) {    // uniform result
+  unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);
+  v = v > o ? v : o;
+  o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);
+  v = v > o ? v : o;
+  o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true);   // row_half_mirror
+  v = v > o ? v : o;
+  o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true);   // row_mirror: all 16 lanes of a row agree
+  v = v > o ? v : o;
+  const unsigned a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
+  const unsigned c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
+  const unsigned ab = a > b ? a : b, cd = c > d ? c : d;
+  return ab > cd ? ab : cd;
+}
+
+__device__ __forceinline__ void wave_join(Stat* st) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) st->join(__shfl_xor(st->m, o, 64), __shfl_xor(st->s, o, 64), __shfl_xor(st->t, o, 64));
+}
+
+// A wave's list of the best classes so far: lane j < top holds the j-th (key, class), best first.  An empty place has
+// key 0, below every number's.
+struct WaveList {
+  unsigned key;
+  int cls;
+  unsigned last_key;     // uniform: the list's last place
+  int last_cls;
+  __device__ __forceinline__ void clear() { key = 0; cls = 0x7fffffff; last_key = 0; last_cls = 0x7fffffff; }
+  __device__ __forceinline__ bool beaten_by(unsigned k, int c) const { return k > last_key || (k == last_key && c < last_cls); }
+  // take a uniform candidate that beats the last place
+  __device__ __forceinline__ void insert(unsigned k, int c, int lane, int top) {
+    const bool before = lane < top && (key > k || (key == k && cls < c));
+    const int pos = __popcll(__ballot(before));
+    const unsigned pk = (unsigned)__builtin_amdgcn_mov_dpp((int)key, 0x111, 0xF, 0xF, true);    // row_shr 1: top <= 16, one row
+    const int pc = __builtin_amdgcn_mov_dpp(cls, 0x111, 0xF, 0xF, true);
+    if (lane > pos) { key = pk; cls = pc; }
+    if (lane == pos) { key = k; cls = c; }
+    last_key = (unsigned)__builtin_amdgcn_readlane((int)key, top - 1);
+    last_cls = __builtin_amdgcn_readlane(cls, top - 1);
+  }
+  // candidates of all lanes at once (k = 0: none)
+  __device__ __forceinline__ void offer(unsigned k, int c, int lane, int top) {
+    unsigned long long who = __ballot(k != 0 && beaten_by(k, c));
+    while (who) {
+      const int l = __ffsll((long long)who) - 1;
+      insert((unsigned)__builtin_amdgcn_readlane((int)k, l), __builtin_amdgcn_readlane(c, l), lane, top);
+      who &= who - 1;
+      who &= __ballot(k != 0 && beaten_by(k, c));
+    }
+  }
+};
+
+__device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+
+// ---------------------------------------------------------------- rows: the classes of a site are adjacent
+// NT threads (one wave, or a workgroup) per row, 16-byte loads with the row's unaligned ends taken one by one.  Bound by
+// HBM for many rows, by the latency of one pass for few: 1024 threads on one row keep 16 loads of 1 KiB in flight.
+//
+// The alternatives cost no second pass: a lane's running maximum is the largest of its own classes, so the `top`-th
+// largest of the lanes' maxima is a lower bound for the top-th best class, and only lanes whose maximum reaches it can
+// hold one.  Those few lanes go over their own classes again (in cache) and offer what reaches the bound to a list.
+template <int DT> struct Vec {
+  typedef typename Elem<DT>::type T;
+  static constexpr int N = 16 / sizeof(T);
+  union { uint4 q; T e[N]; };
+};
+
+struct RowPart {      // how a row's classes are dealt out: head one by one, body in vectors, tail one by one
+  int head, body, tail0;
+};
+template <int DT>
+__device__ __forceinline__ RowPart row_part(const typename Elem<DT>::type* row, int classes) {
+  constexpr int N = Vec<DT>::N;
+  RowPart r;
+  r.head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(typename Elem<DT>::type);
+  r.head = r.head < classes ? r.head : classes;
+  r.body = (classes - r.head) / N;
+  r.tail0 = r.head + r.body * N;
+  return r;
+}
+
+// one vector's worth of classes into a lane's statistics
+template <int N>
+__device__ __forceinline__ void add_many(Stat* st, const float* x) {
+  float vm = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) vm = fmaxf(vm, x[i]);
+  if (vm > st->m) {
+    const float a = __expf(st->m - vm);
+    st->t = a * (st->t + st->s * fmaxf(st->m - vm, kFloor));
+    st->s = a * st->s;
+    st->m = vm;
+  }
+  const float m = st->m == NEG_INF ? 0.f : st->m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = x[i] - m, e = __expf(d);
+    st->s += e;
+    st->t += e * fmaxf(d, kFloor);
+  }
+}
+
+template <int DT, int NT>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void symbol_rows_kernel(Logits l, const int* symbols, int top, float* log_prob,
+                                                                          float* entropy, float* stats, float* top_lp, int* top_sym,
+                                                                          int sites) {
+  typedef typename Elem<DT>::type T;
+  constexpr int N = Vec<DT>::N, WAVES = NT / 64, ROWS = NT < 256 ? 256 / NT : 1;
+  __shared__ float part[WAVES > 1 ? WAVES * 3 : 1];
+  __shared__ unsigned keys[WAVES > 1 ? WAVES * DVC_MAX_TOP : 1];
+  __shared__ int classes_of[WAVES > 1 ? WAVES * DVC_MAX_TOP : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int tid = ROWS > 1 ? lane : (int)threadIdx.x;
+  const int site = __builtin_amdgcn_readfirstlane((int)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0));
+  if (site >= sites) return;            // (whole waves, and only where a row is a wave: no barrier below is missed)
+  const int n = site / l.groups, g = site - n * l.groups;
+  const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes;
+  const RowPart rp = row_part<DT>(row, l.classes);
+  const uint4* const body = reinterpret_cast<const uint4*>(row + rp.head);
+
+  Stat st;
+  st.clear();
+  // ends: at most N - 1 classes on either side
+  const int ends = rp.head + l.classes - rp.tail0;
+  const int end_v = tid < rp.head ? tid : rp.tail0 + tid - rp.head;
+  const bool has_end = tid < ends;
+  const float end_x = has_end ? Elem<DT>::up(row[end_v]) : NEG_INF;
+  if (has_end) st.add(end_x);
+  constexpr int U = 4;
+  int j = tid;
+  for (; j + (U - 1) * NT < rp.body; j += U * NT) {
+    Vec<DT> q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u].q = body[j + u * NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = Elem<DT>::up(q[u].e[i]);
+      add_many<N>(&st, x);
+    }
+  }
+  for (; j < rp.body; j += NT) {
+    Vec<DT> q;
+    q.q = body[j];
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = Elem<DT>::up(q.e[i]);
+    add_many<N>(&st, x);
+  }
+
+  // what the lane's best class is worth; a lane that met a NaN or +inf looks again (its maximum ignores NaN)
+  unsigned best = 0;
+  if (top > 0) {
+    if (has_end || tid < rp.body) best = order_key(st.m);
+    if (st.s != st.s) {
+      if (has_end) best = order_key(end_x);
+      for (int v = tid; v < rp.body; v += NT) {
+        Vec<DT> q;
+        q.q = body[v];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const unsigned k = order_key(Elem<DT>::up(q.e[i]));
+          best = k > best ? k : best;
+        }
+      }
+    }
+  }
+
+  Stat all = st;
+  wave_join(&all);
+  if constexpr (WAVES > 1) {
+    if (lane == 0) { part[wave * 3] = all.m; part[wave * 3 + 1] = all.s; part[wave * 3 + 2] = all.t; }
+  }
+  // the wave's `top` best lanes, one after the other
+  unsigned bound = 0;
+  if (top > 0) {
+    unsigned k = best, mine = 0;
+    for (int i = 0; i < top; ++i) {
+      bound = wave_max(k);
+      if (lane == i) mine = bound;
+      const unsigned long long eq = __ballot(k == bound);
+      if (lane == __ffsll((long long)eq) - 1) k = 0;
+    }
+    if constexpr (WAVES > 1) {
+      if (lane < top) keys[wave * DVC_MAX_TOP + lane] = mine;
+    }
+  }
+  if constexpr (WAVES > 1) {
+    __syncthreads();
+    all.clear();
+    for (int w = 0; w < WAVES; ++w) all.join(part[w * 3], part[w * 3 + 1], part[w * 3 + 2]);
+    if (top > 0) {
+      // the top-th best of all waves' (WAVES * 16 places, in every wave alike)
+      constexpr int PER = (WAVES * DVC_MAX_TOP + 63) / 64;
+      unsigned k[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int at = i * 64 + lane;
+        k[i] = at < WAVES * DVC_MAX_TOP && at % DVC_MAX_TOP < top ? keys[at] : 0;
+      }
+      for (int r = 0; r < top; ++r) {
+        unsigned mx = k[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) mx = k[i] > mx ? k[i] : mx;
+        bound = wave_max(mx);
+        const unsigned long long eq = __ballot(mx == bound);
+        if (lane == __ffsll((long long)eq) - 1) {
+          bool done = false;
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (!done && k[i] == bound) { k[i] = 0; done = true; }
+        }
+      }
+    }
+  }
+  float log_s, h;
+  finish(all, &log_s, &h);
+
+  if (top > 0) {
+    WaveList list;
+    list.clear();
+    const bool in = best >= bound && best != 0;      // (fewer lanes than `top` with a class: bound 0, all look)
+    if (__ballot(in)) {
+      const unsigned ke = order_key(end_x);
+      list.offer(in && has_end && ke >= bound ? ke : 0, end_v, lane, top);
+      for (int v = tid; v - tid + (tid & ~63) < rp.body; v += NT) {      // uniform over the wave
+        Vec<DT> q;
+        const bool have = in && v < rp.body;
+        if (have) q.q = body[v];
+        float vm = NEG_INF;
+        bool nan = false;
+        float x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          x[i] = have ? Elem<DT>::up(q.e[i]) : 0.f;
+          vm = fmaxf(vm, x[i]);
+          nan |= x[i] != x[i];
+        }
+        const unsigned km = nan ? 0xffffffffu : order_key(vm);
+        if (!__ballot(have && km >= bound && km >= list.last_key)) continue;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const unsigned k = order_key(x[i]);
+          list.offer(have && k >= bound ? k : 0, rp.head + v * N + i, lane, top);
+        }
+      }
+    }
+    if constexpr (WAVES > 1) {
+      __syncthreads();                   // the keys of the bound have been read
+      if (lane < top) {
+        keys[wave * DVC_MAX_TOP + lane] = list.key;
+        classes_of[wave * DVC_MAX_TOP + lane] = list.cls;
+      }
+      __syncthreads();
+      if (wave == 0)
+        for (int b = DVC_MAX_TOP; b < WAVES * DVC_MAX_TOP; b += 64) {      // place 0..15 is this wave's own list
+          const int at = b + lane;
+          const bool have = at < WAVES * DVC_MAX_TOP && at % DVC_MAX_TOP < top;
+          list.offer(have ? keys[at] : 0, have ? classes_of[at] : 0, lane, top);
+        }
+    }
+    if ((ROWS > 1 || wave == 0) && lane < top) {
+      top_lp[(long long)site * top + lane] = log_p(key_value(list.key), all.m, log_s);
+      top_sym[(long long)site * top + lane] = list.cls;
+    }
+  }
+  if ((ROWS > 1 || wave == 0) && lane == 0) {
+    log_prob[site] = given<DT>(row, 1, l.classes, symbols[site], all.m, log_s);
+    entropy[site] = h;
+    stats[site] = all.m;
+    stats[(long long)sites + site] = log_s;
+  }
+}
+
+// ---------------------------------------------------------------- planes: the classes of a site are planes apart
+// A lane per site, so a wave reads 64 adjacent pixels of one class at a time.  With few sites the classes are cut into SL
+// ranges, one per wave of the workgroup, joined through LDS.  The alternatives are a short sorted list per thread.
+template <int TOP>
+struct ThreadList {
+  unsigned key[TOP > 0 ? TOP : 1];
+  int cls[TOP > 0 ? TOP : 1];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < TOP; ++j) { key[j] = 0; cls[j] = 0x7fffffff; }
+  }
+  // candidates come in rising class order: an equal key goes behind
+  __device__ __forceinline__ void insert(unsigned k, int c) {
+#pragma unroll
+    for (int j = TOP - 1; j >= 1; --j) {
+      const bool above = k > key[j - 1], here = k > key[j];
+      cls[j] = above ? cls[j - 1] : here ? c : cls[j];
+      key[j] = above ? key[j - 1] : here ? k : key[j];
+    }
+    if (k > key[0]) { key[0] = k; cls[0] = c; }
+  }
+};
+
+template <int DT, int TOP, int SL>
+__global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Logits l, const int* symbols, int top, float* log_prob,
+                                                                              float* entropy, float* stats, float* top_lp,
+                                                                              int* top_sym, long long sites, unsigned hw) {
+  typedef typename Elem<DT>::type T;
+  constexpr int SITES = SL == 1 ? 256 : 64;
+  __shared__ float part[SL > 1 ? SL * 3 * 64 : 1];
+  __shared__ unsigned keys[SL > 1 && TOP > 0 ? SL * TOP * 64 : 1];
+  __shared__ int classes_of[SL > 1 && TOP > 0 ? SL * TOP * 64 : 1];
+  const int slot = threadIdx.x % SITES;
+  const int slice = SL == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x / SITES));
+  const long long i = (long long)blockIdx.x * SITES + slot;
+  const bool live = i < sites;
+  const long long ic = live ? i : sites - 1;             // idle lanes repeat the last site
+  const long long ng = ic / hw;
+  const unsigned p = (unsigned)(ic - ng * hw);
+  const int n = (int)(ng / l.groups), g = (int)(ng - (long long)n * l.groups);
+  const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes * l.cs + p;
+  const int per = (l.classes + SL - 1) / SL;
+  const int v0 = slice * per, v1 = v0 + per < l.classes ? v0 + per : l.classes;
+
+  Stat st;
+  st.clear();
+  ThreadList<TOP> list;
+  list.clear();
+  float last = NEG_INF;
+  auto take = [&](float x, int v) {
+    if constexpr (TOP > 0) {
+      if (v - v0 < TOP || !(x <= last)) {      // (a NaN, or behind one, compares false: the keys decide)
+        list.insert(order_key(x), v);
+        last = list.key[TOP - 1] != 0 ? key_value(list.key[TOP - 1]) : NEG_INF;
+      }
+    }
+  };
+  constexpr int U = 8;
+  int v = v0;
+  for (; v + U <= v1; v += U) {
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = Elem<DT>::up(row[(long long)(v + u) * l.cs]);
+    add_many<U>(&st, x);
+#pragma unroll
+    for (int u = 0; u < U; ++u) take(x[u], v + u);
+  }
+  for (; v < v1; ++v) {
+    const float x = Elem<DT>::up(row[(long long)v * l.cs]);
+    add_many<1>(&st, &x);
+    take(x, v);
+  }
+
+  if constexpr (SL > 1) {
+    part[(slice * 3 + 0) * 64 + slot] = st.m;
+    part[(slice * 3 + 1) * 64 + slot] = st.s;
+    part[(slice * 3 + 2) * 64 + slot] = st.t;
+    if constexpr (TOP > 0)
+#pragma unroll
+      for (int j = 0; j < TOP; ++j) {
+        keys[(slice * TOP + j) * 64 + slot] = list.key[j];
+        classes_of[(slice * TOP + j) * 64 + slot] = list.cls[j];
+      }
+    __syncthreads();
+    if (slice != 0) return;
+    for (int s = 1; s < SL; ++s) {
+      st.join(part[(s * 3 + 0) * 64 + slot], part[(s * 3 + 1) * 64 + slot], part[(s * 3 + 2) * 64 + slot]);
+      if constexpr (TOP > 0)
+        for (int j = 0; j < TOP; ++j) {
+          const unsigned k = keys[(s * TOP + j) * 64 + slot];
+          if (k > list.key[TOP - 1]) list.insert(k, classes_of[(s * TOP + j) * 64 + slot]);
+        }
+    }
+  }
+  if (!live) return;
+  float log_s, h;
+  finish(st, &log_s, &h);
+  log_prob[i] = given<DT>(row, l.cs, l.classes, symbols[i], st.m, log_s);
+  entropy[i] = h;
+  stats[i] = st.m;
+  stats[sites + i] = log_s;
+  if constexpr (TOP > 0)
+#pragma unroll
+    for (int j = 0; j < TOP; ++j)
+      if (j < top) {
+        const long long at = (ng * top + j) * hw + p;
+        top_lp[at] = log_p(key_value(list.key[j]), st.m, log_s);
+        top_sym[at] = list.cls[j];
+      }
+}
+
+// ---------------------------------------------------------------- gradient: one read, one write
+struct SiteGrad {
+  float m, log_s, h, a, b;
+  int sym;
+  __device__ __forceinline__ void load(const Logits& l, const int* symbols, const float* stats, const float* entropy, const float* g_lp,
+                                       const float* g_h, long long i, long long sites) {
+    sym = symbols[i];
+    m = stats[i];
+    m = m == NEG_INF ? 0.f : m;
+    log_s = stats[sites + i];
+    h = entropy[i];
+    a = g_lp != nullptr && sym >= 0 ? (sym < l.classes ? g_lp[i] : __uint_as_float(0x7fc00000u)) : 0.f;
+    b = g_h != nullptr ? g_h[i] : 0.f;
+  }
+  __device__ __forceinline__ float of(float x, int v) const {
+    const float lp = (x - m) - log_s, pv = __expf(lp);
+    const float d = -pv * (a + b * (fmaxf(lp, kFloor) + h));
+    return v == sym ? d + a : d;
+  }
+};
+
+constexpr int kRowVecs = 4;      // vectors per thread of the row form
+
+template <int DT>
+__global__ __launch_bounds__(256) void symbol_rows_backward_kernel(Logits l, const int* symbols, const float* stats, const float* entropy,
+                                                                   const float* g_lp, const float* g_h,
+                                                                   typename Elem<DT>::type* grad, int sites, int chunks) {
+  typedef typename Elem<DT>::type T;
+  constexpr int N = Vec<DT>::N;
+  const int site = (int)(blockIdx.x / (unsigned)chunks), chunk = (int)(blockIdx.x - (unsigned)site * chunks);
+  const int n = site / l.groups, g = site - n * l.groups;
+  const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes;
+  T* const out = grad + (long long)site * l.classes;
+  SiteGrad sg;
+  sg.load(l, symbols, stats, entropy, g_lp, g_h, site, sites);
+  RowPart rp = row_part<DT>(row, l.classes);
+  const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;   // one vector grid for both
+  const int j0 = chunk * 256 * kRowVecs + threadIdx.x;
+  if (chunk == 0) {
+    const int ends = rp.head + l.classes - rp.tail0;
+    if ((int)threadIdx.x < ends) {
+      const int v = (int)threadIdx.x < rp.head ? (int)threadIdx.x : rp.tail0 + (int)threadIdx.x - rp.head;
+      out[v] = Elem<DT>::down(sg.of(Elem<DT>::up(row[v]), v));
+    }
+  }
+  const uint4* const body = reinterpret_cast<const uint4*>(row + rp.head);
+  Vec<DT> q[kRowVecs];
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u)
+    if (j0 + u * 256 < rp.body) q[u].q = body[j0 + u * 256];
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) {
+    const int j = j0 + u * 256;
+    if (j < rp.body) {
+      const int v = rp.head + j * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) q[u].e[i] = Elem<DT>::down(sg.of(Elem<DT>::up(q[u].e[i]), v + i));
+      if (together) {
+        reinterpret_cast<uint4*>(out + rp.head)[j] = q[u].q;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[v + i] = q[u].e[i];
+      }
+    }
+  }
+}
+
+constexpr int kPlaneClasses = 16;      // classes per thread of the plane form
+
+template <int DT>
+__global__ __launch_bounds__(256) void symbol_planes_backward_kernel(Logits l, const int* symbols, const float* stats,
+                                                                     const float* entropy, const float* g_lp, const float* g_h,
+                                                                     typename Elem<DT>::type* grad, long long sites, unsigned hw,
+                                                                     unsigned chunks) {
+  typedef typename Elem<DT>::type T;
+  const unsigned blk = blockIdx.x / chunks, chunk = blockIdx.x - blk * chunks;
+  const long long i = (long long)blk * 256 + threadIdx.x;
+  if (i >= sites) return;
+  const long long ng = i / hw;
+  const unsigned p = (unsigned)(i - ng * hw);
+  const int n = (int)(ng / l.groups), g = (int)(ng - (long long)n * l.groups);
+  const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes * l.cs + p;
+  T* const out = grad + ng * l.classes * hw + p;
+  SiteGrad sg;
+  sg.load(l, symbols, stats, entropy, g_lp, g_h, i, sites);
+  const int v0 = (int)chunk * kPlaneClasses;
+  T q[kPlaneClasses];
+#pragma unroll
+  for (int u = 0; u < kPlaneClasses; ++u)
+    if (v0 + u < l.classes) q[u] = row[(long long)(v0 + u) * l.cs];
+#pragma unroll
+  for (int u = 0; u < kPlaneClasses; ++u)
+    if (v0 + u < l.classes) out[(long long)(v0 + u) * hw] = Elem<DT>::down(sg.of(Elem<DT>::up(q[u]), v0 + u));
+}
+
+int check_logits(const DvcLogits* l, int batch, int h, int w, const char* who) {
+  DVC_REQUIRE(l != nullptr && l->ptr != nullptr, "%s: null logits", who);
+  DVC_REQUIRE(l->groups >= 1 && l->classes >= 1, "%s: bad groups / classes (%d, %d)", who, l->groups, l->classes);
+  DVC_REQUIRE(l->dtype == DVC_F32 || l->dtype == DVC_BF16 || l->dtype == DVC_F16, "%s: type %d unknown", who, l->dtype);
+  DVC_REQUIRE(batch >= 1 && h >= 1 && w >= 1, "%s: bad dims", who);
+  DVC_REQUIRE((long long)h * w < (1LL << 28), "%s: plane too large", who);
+  DVC_REQUIRE((long long)batch * l->groups < (1LL << 31), "%s: too many groups", who);
+  DVC_REQUIRE(l->class_stride >= (int64_t)h * w, "%s: class stride < H*W", who);
+  return DVC_OK;
+}
+inline Logits mk(const DvcLogits* l) { return Logits{l->ptr, l->batch_stride, l->class_stride, l->groups, l->classes}; }
+
+// The classes of a site are adjacent: one pixel per plane and unit class stride (groups follow each other).
+inline bool is_rows(const DvcLogits* l, int h, int w) {
+  return h == 1 && w == 1 && (l->class_stride == 1 || (l->classes == 1 && l->groups == 1));
+}
+
+template <int DT>
+int launch_forward(const DvcLogits* l, const int32_t* symbols, int top, float* log_prob, float* entropy, float* stats, float* top_lp,
+                   int32_t* top_sym, int batch, int h, int w, hipStream_t st) {
+  const unsigned hw = (unsigned)((long long)h * w);
+  const long long sites = (long long)batch * l->groups * hw;
+  if (is_rows(l, h, w)) {
+#define ROWS(NT, GRID, BLOCK) hipLaunchKernelGGL((symbol_rows_kernel<DT, NT>), dim3(GRID), dim3(BLOCK), 0, st, mk(l), symbols, top, log_prob, \
+                                                 entropy, stats, top_lp, top_sym, (int)sites)
+    // A wave per row while a row is at most a few vectors per lane; otherwise a workgroup: of 16 waves where the rows
+    // alone do not fill the 256 CUs (fewer than 1024 of them) and a row gives every lane a vector
+    if (l->classes <= 1024) ROWS(64, (unsigned)((sites + 3) / 4), 256);
+    else if (sites >= 1024 || l->classes < 8192) ROWS(256, (unsigned)sites, 256);
+    else ROWS(1024, (unsigned)sites, 1024);
+#undef ROWS
+    return dvc::check_launch("symbol_rows_kernel");
+  }
+  const long long waves = (sites + 63) / 64;
+  DVC_REQUIRE(waves < (1LL << 31), "dvc_symbol_log_probs: too many sites");
+#define PLANES(TOP, SL) hipLaunchKernelGGL((symbol_planes_kernel<DT, TOP, SL>), dim3((unsigned)((sites + (SL == 1 ? 255 : 63)) / (SL == 1 ? 256 : 64))), \
+                                           dim3(SL == 1 ? 256 : 64 * SL), 0, st, mk(l), symbols, top, log_prob, entropy, stats, top_lp,      \
+                                           top_sym, sites, hw)
+  // Cut the classes while the sites alone give fewer than eight waves per CU and a range keeps eight classes; the joining
+  // lists of 16 ranges fit LDS up to 4 alternatives
+#define SLICES(TOP)                                                                        \
+  do {                                                                                     \
+    if (TOP <= 4 && waves < 512 && l->classes >= 128) PLANES(TOP, (TOP <= 4 ? 16 : 4));    \
+    else if (waves < 2048 && l->classes >= 32) PLANES(TOP, 4);                             \
+    else PLANES(TOP, 1);                                                                   \
+  } while (0)
+  if (top == 0) SLICES(0);
+  else if (top == 1) SLICES(1);
+  else if (top <= 4) SLICES(4);
+  else if (top <= 8) SLICES(8);
+  else SLICES(16);
+#undef SLICES
+#undef PLANES
+  return dvc::check_launch("symbol_planes_kernel");
+}
+
+template <int DT>
+int launch_backward(const DvcLogits* l, const int32_t* symbols, const float* stats, const float* entropy, const float* g_lp,
+                    const float* g_h, void* grad, int batch, int h, int w, hipStream_t st, const char* who) {
+  typedef typename Elem<DT>::type T;
+  const unsigned hw = (unsigned)((long long)h * w);
+  const long long sites = (long long)batch * l->groups * hw;
+  if (is_rows(l, h, w)) {
+    const int per = 256 * kRowVecs * Vec<DT>::N;
+    const long long chunks = (l->classes + per - 1) / per;
+    DVC_REQUIRE(sites * chunks < (1LL << 31), "%s: too many sites", who);
+    hipLaunchKernelGGL(symbol_rows_backward_kernel<DT>, dim3((unsigned)(sites * chunks)), dim3(256), 0, st, mk(l), symbols, stats, entropy,
+                       g_lp, g_h, static_cast<T*>(grad), (int)sites, (int)chunks);
+    return dvc::check_launch("symbol_rows_backward_kernel");
+  }
+  const long long chunks = (l->classes + kPlaneClasses - 1) / kPlaneClasses, blocks = (sites + 255) / 256;
+  DVC_REQUIRE(blocks * chunks < (1LL << 31), "%s: too many sites", who);
+  hipLaunchKernelGGL(symbol_planes_backward_kernel<DT>, dim3((unsigned)(blocks * chunks)), dim3(256), 0, st, mk(l), symbols, stats, entropy,
+                     g_lp, g_h, static_cast<T*>(grad), sites, hw, (unsigned)chunks);
+  return dvc::check_launch("symbol_planes_backward_kernel");
+}
+
+}  // namespace
+
+extern "C" int64_t dvc_symbol_log_probs_scratch_floats(const DvcLogits* logits, int32_t top, int32_t batch, int32_t h, int32_t w) {
+  if (int rc = check_logits(logits, batch, h, w, "dvc_symbol_log_probs_scratch_floats")) return rc;
+  return 0;
+}
+
+extern "C" int dvc_symbol_log_probs(const DvcLogits* logits, const int32_t* symbols, int32_t top, float* log_prob, float* entropy,
+                                    float* stats, float* top_log_prob, int32_t* top_symbol, float* scratch, int32_t batch,
+                                    int32_t h, int32_t w, void* stream) {
+  if (int rc = check_logits(logits, batch, h, w, "dvc_symbol_log_probs")) return rc;
+  DVC_REQUIRE(symbols != nullptr && log_prob != nullptr && entropy != nullptr && stats != nullptr, "dvc_symbol_log_probs: null pointer");
+  DVC_REQUIRE(top >= 0 && top <= DVC_MAX_TOP && top <= logits->classes, "dvc_symbol_log_probs: top=%d (0..%d, at most the %d classes)",
+              top, DVC_MAX_TOP, logits->classes);
+  DVC_REQUIRE(top == 0 || (top_log_prob != nullptr && top_symbol != nullptr), "dvc_symbol_log_probs: null pointer");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define GO(DT) launch_forward<DT>(logits, symbols, top, log_prob, entropy, stats, top_log_prob, top_symbol, batch, h, w, st)
+  return logits->dtype == DVC_F32 ? GO(DVC_F32) : logits->dtype == DVC_BF16 ? GO(DVC_BF16) : GO(DVC_F16);
+#undef GO
+}
+
+extern "C" int dvc_symbol_log_probs_backward(const DvcLogits* logits, const int32_t* symbols, const float* stats, const float* entropy,
+                                             const float* grad_log_prob, const float* grad_entropy, void* grad_logits, int32_t batch,
+                                             int32_t h, int32_t w, void* stream) {
+  const char* const who = "dvc_symbol_log_probs_backward";
+  if (int rc = check_logits(logits, batch, h, w, who)) return rc;
+  DVC_REQUIRE(symbols != nullptr && stats != nullptr && entropy != nullptr && grad_logits != nullptr, "%s: null pointer", who);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define GO(DT) launch_backward<DT>(logits, symbols, stats, entropy, grad_log_prob, grad_entropy, grad_logits, batch, h, w, st, who)
+  return logits->dtype == DVC_F32 ? GO(DVC_F32) : logits->dtype == DVC_BF16 ? GO(DVC_BF16) : GO(DVC_F16);
+#undef GO
+}

@@ -39,6 +39,8 @@ class Conv2d(nn.Module):
         self.precision = 0      # ops.PRECISIONS: 0 exact fp32, 1 bf16, 2 bf16 hi + lo split, 3 fp16 hi + lo split
         # the same for the forward and data-gradient convolutions under autograd (DMC.set_precision(..., train=True))
         self.train_precision = 0
+        # what the tape keeps of this layer's operands: None fp32, "int8" / "e4m3" 8-bit checkpoints (DMC.set_act_storage)
+        self.act_storage: Optional[str] = None
 
     def _precision(self) -> int:
         # layers with a handful of output channels (the flow and RGB heads) run on the vector ALUs in exact fp32
@@ -84,7 +86,7 @@ class Conv2d(nn.Module):
             return A.conv2d(x, self.weight, self.bias, stride=self.stride, in_slope=in_slope, out_slope=out_slope,
                             residual=residual, res_scale=res_scale, residual2=residual2,
                             pixel_shuffle=pixel_shuffle, packed=self.packed_weight(pf), dgrad_packed=self.dgrad_weight(pd),
-                            precision=pf, dgrad_precision=pd)
+                            precision=pf, dgrad_precision=pd, storage=self.act_storage)
         return ops.conv2d(x, self.weight.detach(), self.bias.detach(), stride=self.stride, in_slope=in_slope,
                           out_slope=out_slope, residual=residual, res_scale=res_scale, residual2=residual2,
                           pixel_shuffle=pixel_shuffle, out=out, packed=self.packed_weight(self._precision()),
@@ -207,10 +209,11 @@ class SELayer(nn.Module):
         lin1 = nn.Linear(channel, channel // reduction, bias=False)
         lin2 = nn.Linear(channel // reduction, channel, bias=False)
         self.fc = Indexed(_0=lin1, _2=lin2)  # parameter names fc.0.weight / fc.2.weight
+        self.act_storage: Optional[str] = None      # as in Conv2d
 
     def forward(self, x: Tensor) -> Tensor:
         if torch.is_grad_enabled():
-            return A.se_gate(x, self.fc[0].weight, self.fc[2].weight)
+            return A.se_gate(x, self.fc[0].weight, self.fc[2].weight, self.act_storage)
         return ops.se_gate(x, self.fc[0].weight.detach(), self.fc[2].weight.detach())
 
     def from_sums(self, sums: Tensor, h: int, w: int) -> Tensor:

@@ -23,11 +23,11 @@ import numpy as np
 import torch
 import torch.nn as nn
 
+from .. import _lib, ops
 from .. import autograd as A
-from .. import ops
 from .base_model import CompressionModel, get_scale_table
 from .entropy_models import GaussianConditional, uniform_noise
-from .layers import (ConvStack3, Conv2d, Indexed, ME_Spynet, ResBlock, UNet, bilineardownsacling, flow_warp,
+from .layers import (ConvStack3, Conv2d, Indexed, ME_Spynet, ResBlock, SELayer, UNet, bilineardownsacling, flow_warp,
                      get_enc_dec_models, get_hyper_enc_dec_models, subpel_conv3x3)
 from .utils import resize_registered_buffers
 
@@ -670,6 +670,19 @@ class DMC(nn.Module):
                     m.train_precision = ops.PRECISIONS[precision]
                 else:
                     m.precision = ops.PRECISIONS[precision]
+        return self
+
+    def set_act_storage(self, storage: str = "fp32"):
+        """What the tape of a training step keeps of the convolutions' operands: "fp32" (default) the tensors
+        themselves; "int8" or "e4m3" 8-bit checkpoints with one power-of-two scale per 32 adjacent values of a channel
+        plane, and one bit per value where only an activation's derivative is needed.  The forward pass and the data and
+        bias gradients do not change; a weight gradient is that of the stored operand (int8: off by at most half of
+        1/127..1/63 of the block's largest magnitude, e4m3: by at most 1/16 of each value)."""
+        if storage != "fp32" and storage not in _lib.CKPT_FORMATS:
+            raise ValueError(f"unknown activation storage {storage!r} (fp32, {', '.join(_lib.CKPT_FORMATS)})")
+        for m in self.modules():
+            if isinstance(m, (Conv2d, SELayer)):
+                m.act_storage = None if storage == "fp32" else storage
         return self
 
     def aux_loss(self):

@@ -2,17 +2,17 @@
 
 torch is used for device memory and stream plumbing only: every arithmetic op
 here is a HIP kernel of this package launched on torch's current stream.
-All tensors must be fp32 (int32 for symbols / indexes) CUDA(HIP) tensors in
-NCHW with contiguous rows; batch / channel strides are free, so channel slices
+All tensors must be fp32 (int32 for symbols / indexes, uint8 for 8-bit checkpoints;
+logits may be bf16 / fp16 as well) CUDA(HIP) tensors in NCHW with contiguous rows; batch / channel strides are free, so channel slices
 of a larger buffer are accepted as sources, residuals and destinations.
 """
 import ctypes as C
-from typing import Optional, Sequence, Tuple, Union
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import DvcConv2d, DvcDst, DvcSrc, check
+from ._lib import DvcCkpt, DvcConv2d, DvcDst, DvcLogits, DvcSrc, check
 
 Tensor = torch.Tensor
 Srcs = Union[Tensor, Sequence[Tensor]]
@@ -609,4 +609,251 @@ def sq_err_backward(a: Tensor, b: Tensor, grad_sse: Tensor) -> Tensor:
     out = torch.empty((n, c, h, w), dtype=torch.float32, device=a.device)
     check(_lib.load().dvc_sq_err_backward(C.byref(_src(a, "a")), C.byref(_src(b, "b")), grad_sse.data_ptr(),
                                           C.byref(_dst(out)), n, h, w, _stream()), "dvc_sq_err_backward")
+    return out
+
+
+# ------------------------------------------------------------------------------------ 8-bit activation checkpoints
+class ActCheckpoint(NamedTuple):
+    """An activation kept in 8 bits between the forward and the backward pass (format: include/dvc_hip.h): one byte
+    per value and one power-of-two scale per 32 adjacent values of a channel plane."""
+    codes: Tensor        # uint8 (N, C, blocks * 32), contiguous
+    scales: Tensor       # uint8 (N, C, blocks), contiguous
+    shape: Tuple[int, int, int, int]
+    fmt: str             # "int8" or "e4m3"
+
+
+def _blocks(h: int, w: int) -> int:
+    return (h * w + 31) // 32
+
+
+def _on_current_device(t: Tensor, name: str):
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _ckpt_format(fmt: str) -> int:
+    if fmt not in _lib.CKPT_FORMATS:
+        raise ValueError(f"unknown checkpoint format {fmt!r} (one of {', '.join(_lib.CKPT_FORMATS)})")
+    return _lib.CKPT_FORMATS[fmt]
+
+
+def _ckpt(ck: ActCheckpoint, name: str, device=None) -> DvcCkpt:
+    if not isinstance(ck, ActCheckpoint):
+        raise TypeError(f"{name}: expected an ActCheckpoint, got {type(ck)}")
+    fmt = _ckpt_format(ck.fmt)
+    n, c, h, w = ck.shape
+    if min(n, c, h, w) < 1:
+        raise ValueError(f"{name}: empty shape {tuple(ck.shape)}")
+    _check_vec(ck.codes, n * c * _blocks(h, w) * 32, f"{name} codes", dtype=torch.uint8, device=device)
+    _check_vec(ck.scales, n * c * _blocks(h, w), f"{name} scales", dtype=torch.uint8, device=ck.codes.device)
+    _on_current_device(ck.codes, name)
+    return DvcCkpt(ck.codes.data_ptr(), ck.scales.data_ptr(), c, fmt)
+
+
+def _slope(slope: float, name: str) -> float:
+    """LeakyReLU slopes outside [0, 1] do not keep the sign a derivative is read off (nor max(x, slope x))."""
+    if not 0.0 <= float(slope) <= 1.0:
+        raise ValueError(f"{name}: slope {slope} outside [0, 1]")
+    return float(slope)
+
+
+def act_checkpoint(x: Tensor, slope: Optional[float] = None, fmt: str = "int8") -> ActCheckpoint:
+    """The 8-bit checkpoint of x, or of LeakyReLU(slope)(x) (0.0: ReLU), in `fmt`: "int8" (127 steps of the block's
+    largest magnitude) or "e4m3" (4 significant bits each).  act_restore() gives the values back; the weight gradient
+    (conv2d_wgrad_ckpt) and the input activation's derivative (mul_act_grad_ckpt) read the codes themselves."""
+    code = _ckpt_format(fmt)
+    src = _src(x, "act_checkpoint x")
+    _on_current_device(x, "act_checkpoint x")
+    n, c, h, w = x.shape
+    codes = torch.empty((n, c, _blocks(h, w) * 32), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((n, c, _blocks(h, w)), dtype=torch.uint8, device=x.device)
+    check(_lib.load().dvc_act_checkpoint(C.byref(src), 0 if slope is None else 1,
+                                         1.0 if slope is None else _slope(slope, "act_checkpoint"), code, codes.data_ptr(),
+                                         scales.data_ptr(), n, h, w, _stream()), "dvc_act_checkpoint")
+    return ActCheckpoint(codes, scales, (n, c, h, w), fmt)
+
+
+def act_restore(ck: ActCheckpoint, out: Optional[Tensor] = None) -> Tensor:
+    """The fp32 tensor a checkpoint stands for."""
+    c = _ckpt(ck, "act_restore")
+    n, _, h, w = ck.shape
+    if out is None:
+        out = torch.empty(ck.shape, dtype=torch.float32, device=ck.codes.device)
+    elif tuple(out.shape) != tuple(ck.shape):
+        raise ValueError(f"act_restore: out shape {tuple(out.shape)} != {tuple(ck.shape)}")
+    dst = _dst(out)
+    if out.device != ck.codes.device:
+        raise ValueError(f"act_restore: out on {out.device}, the checkpoint is on {ck.codes.device}")
+    check(_lib.load().dvc_act_restore(C.byref(c), C.byref(dst), n, h, w, _stream()), "dvc_act_restore")
+    return out
+
+
+def act_signs(x: Tensor) -> Tensor:
+    """One bit per value, x > 0, as int32 words of 32 adjacent values of a channel plane: (N, C, blocks)."""
+    src = _src(x, "act_signs x")
+    _on_current_device(x, "act_signs x")
+    n, c, h, w = x.shape
+    signs = torch.empty((n, c, _blocks(h, w)), dtype=torch.int32, device=x.device)
+    check(_lib.load().dvc_act_signs(C.byref(src), signs.data_ptr(), n, h, w, _stream()), "dvc_act_signs")
+    return signs
+
+
+def act_grad_signs(grad: Tensor, signs: Tensor, slope: float, pixel_shuffle: bool, conv_shape) -> Tensor:
+    """act_grad() with the activation's output given by its signs (act_signs of the stored tensor)."""
+    n, c, ho, wo = conv_shape
+    stored = (n, c // 4, 2 * ho, 2 * wo) if pixel_shuffle else (n, c, ho, wo)
+    if tuple(grad.shape) != stored or (pixel_shuffle and c % 4):
+        raise ValueError(f"act_grad_signs: grad shape {tuple(grad.shape)} != {stored}")
+    src = _src(grad, "act_grad_signs grad")
+    _on_current_device(grad, "act_grad_signs grad")
+    _check_vec(signs, n * stored[1] * _blocks(*stored[2:]), "act_grad_signs signs", dtype=torch.int32, device=grad.device)
+    out = torch.empty((n, c, ho, wo), dtype=torch.float32, device=grad.device)
+    check(_lib.load().dvc_act_grad_signs(C.byref(src), signs.data_ptr(), float(slope), 1 if pixel_shuffle else 0,
+                                         out.data_ptr(), n, c, ho, wo, _stream()), "dvc_act_grad_signs")
+    return out
+
+
+def mul_act_grad_ckpt(grad: Tensor, ck: ActCheckpoint, slope: float, out: Optional[Tensor] = None,
+                      plus: Optional[Tensor] = None) -> Tensor:
+    """mul_act_grad() with x given by its checkpoint: grad * (x > 0 ? 1 : slope) (+ plus)."""
+    n, c, h, w = grad.shape
+    if tuple(ck.shape) != (n, c, h, w):
+        raise ValueError(f"mul_act_grad_ckpt: checkpoint shape {tuple(ck.shape)} != {(n, c, h, w)}")
+    if out is None:
+        out = torch.empty((n, c, h, w), dtype=torch.float32, device=grad.device)
+    for t, name in ((out, "out"), (plus, "plus")):
+        if t is not None and (tuple(t.shape) != (n, c, h, w) or t.device != grad.device):
+            raise ValueError(f"mul_act_grad_ckpt: {name} {tuple(t.shape)} on {t.device} does not match grad {(n, c, h, w)}")
+    check(_lib.load().dvc_mul_act_grad_ckpt(C.byref(_src(grad, "grad")), C.byref(_ckpt(ck, "mul_act_grad_ckpt", grad.device)),
+                                            float(slope), C.byref(_src(plus, "plus")) if plus is not None else None,
+                                            C.byref(_dst(out)), n, h, w, _stream()), "dvc_mul_act_grad_ckpt")
+    return out
+
+
+def conv2d_wgrad_ckpt(cks: Union[ActCheckpoint, Sequence[ActCheckpoint]], grad_pre: Tensor, wshape, stride: int = 1,
+                      with_bias: bool = False):
+    """conv2d_wgrad() with the (activated, concatenated) sources given by checkpoints of one format."""
+    if isinstance(cks, ActCheckpoint):
+        cks = (cks,)
+    if not 1 <= len(cks) <= _lib.DVC_MAX_SRC:
+        raise ValueError(f"conv2d_wgrad_ckpt: {len(cks)} sources (1..{_lib.DVC_MAX_SRC} supported)")
+    cout, cin, k, k2 = wshape
+    n, _, h, w = cks[0].shape
+    for i, ck in enumerate(cks):
+        if (ck.shape[0], ck.shape[2], ck.shape[3]) != (n, h, w) or ck.fmt != cks[0].fmt:
+            raise ValueError(f"conv2d_wgrad_ckpt: source {i} ({tuple(ck.shape)}, {ck.fmt}) does not match {(n, '*', h, w)}, {cks[0].fmt}")
+    if sum(ck.shape[1] for ck in cks) != cin or k != k2:
+        raise ValueError(f"conv2d_wgrad_ckpt: weight shape {tuple(wshape)} does not match {sum(ck.shape[1] for ck in cks)} input channels")
+    pad = k // 2
+    want = (n, cout, (h + 2 * pad - k) // stride + 1, (w + 2 * pad - k) // stride + 1)
+    if tuple(grad_pre.shape) != want:
+        raise ValueError(f"conv2d_wgrad_ckpt: grad_pre shape {tuple(grad_pre.shape)} != {want}")
+    _check_vec(grad_pre, None, "conv2d_wgrad_ckpt grad_pre", device=cks[0].codes.device)
+    arr = (DvcCkpt * len(cks))(*[_ckpt(ck, f"conv2d_wgrad_ckpt source {i}", grad_pre.device) for i, ck in enumerate(cks)])
+    lib = _lib.load()
+    nfl = check(lib.dvc_conv2d_wgrad_ckpt_scratch_floats(cout, cin, k, stride, n, h, w), "dvc_conv2d_wgrad_ckpt_scratch_floats")
+    scratch = torch.empty(nfl, dtype=torch.float32, device=grad_pre.device)
+    gw = torch.empty((cout, cin, k, k), dtype=torch.float32, device=grad_pre.device)
+    gb = torch.empty(cout, dtype=torch.float32, device=grad_pre.device) if with_bias else None
+    check(lib.dvc_conv2d_wgrad_ckpt(arr, len(cks), n, h, w, grad_pre.data_ptr(), cout, k, stride, scratch.data_ptr(),
+                                    gw.data_ptr(), _ptr(gb), _stream()), "dvc_conv2d_wgrad_ckpt")
+    return (gw, gb) if with_bias else gw
+
+
+# ------------------------------------------------------------------------------------ symbols under given logits
+class SymbolLogProbs(NamedTuple):
+    """log_prob / entropy: fp32, shaped like the symbols; stats: (2, sites), for symbol_log_probs_backward;
+    top_log_prob / top_symbol: fp32 / int32 (N, C * top, h, w) (rows: (N, top)), or None."""
+    log_prob: Tensor
+    entropy: Tensor
+    stats: Tensor
+    top_log_prob: Optional[Tensor]
+    top_symbol: Optional[Tensor]
+
+
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _logits(logits: Tensor, symbols: Tensor, name: str):
+    """-> (DvcLogits or None without sites, n, groups, h, w, 2-D?)"""
+    for t, what in ((logits, "logits"), (symbols, "symbols")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} {what}: expected a tensor, got {type(t)}")
+        if not t.is_cuda:
+            raise _lib.DvcError(f"{name} {what}: tensor is on {t.device}; the HIP path needs a GPU tensor (no CPU fallback)")
+    if logits.dtype not in _LOGIT_TYPES:
+        raise TypeError(f"{name} logits: expected fp32, bf16 or fp16, got {logits.dtype}")
+    rows = logits.dim() == 2
+    if rows:
+        if symbols.dim() != 1:
+            raise ValueError(f"{name}: symbols {tuple(symbols.shape)} do not match logits {tuple(logits.shape)}")
+        n, groups, h, w = logits.size(0), 1, 1, 1
+        v, bs, cs = logits.size(1), logits.stride(0), logits.stride(1)
+    else:
+        if logits.dim() != 4 or symbols.dim() != 4:
+            raise ValueError(f"{name}: expected logits (N, C * classes, h, w) with symbols (N, C, h, w), or (N, classes) with (N,), "
+                             f"got {tuple(logits.shape)} with {tuple(symbols.shape)}")
+        n, groups, h, w = symbols.shape
+        v = logits.size(1) // max(1, groups)
+        if logits.size(3) > 1 and logits.stride(3) != 1 or logits.size(2) > 1 and logits.stride(2) != logits.size(3):
+            raise ValueError(f"{name} logits: rows must be contiguous (strides {logits.stride()})")
+        bs, cs = logits.stride(0), logits.stride(1)
+    want = (n, v) if rows else (n, groups * v, h, w)
+    if tuple(logits.shape) != want or tuple(symbols.shape) != ((n,) if rows else (n, groups, h, w)) or groups < 1 or v < 1:
+        raise ValueError(f"{name}: symbols {tuple(symbols.shape)} do not match logits {tuple(logits.shape)}")
+    if logits.size(1) == 1:
+        cs = h * w
+    _check_vec(symbols, None, f"{name} symbols", dtype=torch.int32, device=logits.device)
+    _on_current_device(logits, f"{name} logits")
+    if n * h * w == 0:
+        return None, n, groups, h, w, rows
+    return DvcLogits(logits.data_ptr(), bs, cs, groups, v, _LOGIT_TYPES[logits.dtype], 0), n, groups, h, w, rows
+
+
+def symbol_log_probs(logits: Tensor, symbols: Tensor, top: int = 0) -> SymbolLogProbs:
+    """Log probabilities (nats) of given symbols under softmax(logits), the distributions' entropies and, for `top` > 0
+    (at most 16), the `top` most likely classes in falling order (equal logits: the lower class first).
+
+    logits (N, C * classes, h, w), symbols (N, C, h, w) int32: channel c's classes are the channels c * classes ...;
+    or rows, logits (N, classes), symbols (N,).  fp32, bf16 or fp16 logits with free batch and class strides; sums are
+    fp32.  A symbol < 0 means "none here" (log probability 0); one past the last class gives NaN.  Classes that may not
+    occur have logits of -inf; a site without any other has log probability -inf and entropy 0."""
+    lg, n, groups, h, w, rows = _logits(logits, symbols, "symbol_log_probs")
+    dev = logits.device
+    classes = logits.size(1) // groups
+    top = int(top)
+    if not 0 <= top <= min(_lib.MAX_TOP, classes):
+        raise ValueError(f"symbol_log_probs: top={top} (0..{_lib.MAX_TOP}, at most the {classes} classes)")
+    site = tuple(symbols.shape)
+    log_prob = torch.empty(site, dtype=torch.float32, device=dev)
+    entropy = torch.empty(site, dtype=torch.float32, device=dev)
+    stats = torch.empty((2, symbols.numel()), dtype=torch.float32, device=dev)
+    tl = ts = None
+    if top:
+        shape = (n, top) if rows else (n, groups * top, h, w)
+        tl = torch.empty(shape, dtype=torch.float32, device=dev)
+        ts = torch.empty(shape, dtype=torch.int32, device=dev)
+    if lg is not None:
+        lib = _lib.load()
+        nfl = check(lib.dvc_symbol_log_probs_scratch_floats(C.byref(lg), top, n, h, w), "dvc_symbol_log_probs_scratch_floats")
+        scratch = torch.empty(nfl, dtype=torch.float32, device=dev) if nfl else None
+        check(lib.dvc_symbol_log_probs(C.byref(lg), symbols.data_ptr(), top, log_prob.data_ptr(), entropy.data_ptr(),
+                                       stats.data_ptr(), _ptr(tl), _ptr(ts), _ptr(scratch), n, h, w, _stream()), "dvc_symbol_log_probs")
+    return SymbolLogProbs(log_prob, entropy, stats, tl, ts)
+
+
+def symbol_log_probs_backward(logits: Tensor, symbols: Tensor, stats: Tensor, entropy: Tensor,
+                              grad_log_prob: Optional[Tensor], grad_entropy: Optional[Tensor]) -> Tensor:
+    """The gradient with respect to the logits (contiguous, their type) of what symbol_log_probs returned."""
+    lg, n, groups, h, w, rows = _logits(logits, symbols, "symbol_log_probs_backward")
+    dev, sites = logits.device, symbols.numel()
+    _check_vec(stats, 2 * sites, "symbol_log_probs_backward stats", device=dev)
+    _check_vec(entropy, sites, "symbol_log_probs_backward entropy", device=dev)
+    _check_vec(grad_log_prob, sites, "symbol_log_probs_backward grad_log_prob", device=dev)
+    _check_vec(grad_entropy, sites, "symbol_log_probs_backward grad_entropy", device=dev)
+    out = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev)
+    if lg is not None:
+        check(_lib.load().dvc_symbol_log_probs_backward(C.byref(lg), symbols.data_ptr(), stats.data_ptr(), entropy.data_ptr(),
+                                                        _ptr(grad_log_prob), _ptr(grad_entropy), out.data_ptr(), n, h, w, _stream()),
+              "dvc_symbol_log_probs_backward")
     return out

@@ -369,6 +369,85 @@ int dvc_sq_err_backward(const DvcSrc* a, const DvcSrc* b, const float* grad_sse,
                         int32_t batch, int32_t h, int32_t w, void* stream);
 
 /*
+ * ---- 8-bit activation checkpoints: what a training step keeps of an activation between its forward and its
+ * backward pass (the reference keeps fp32 tensors on torch.autograd's tape, dmc/train.py:329-336).
+ *
+ * Every channel plane (h*w values, row after row) is cut into blocks of 32.  A block has one scale 2^(s - 127), s a
+ * byte: the smallest power of two that holds the block's largest magnitude (in 127 integer steps, DVC_CKPT_INT8, or
+ * in the 448 of OCP e4m3, DVC_CKPT_E4M3), s >= 17; s = 255 marks a block with an infinity or NaN: all of it restores
+ * to NaN.  A code is a byte: bit 7 = "not greater than zero" (set for zero as well, so that an activation's derivative
+ * is read off the code alone, also where the magnitude rounded to zero), the low seven bits the magnitude, rounded
+ * to nearest even (in the topmost binade down where up would be 2^128).  The last block of a plane is filled with code 128.  codes are contiguous (batch, channels,
+ * blocks * 32), scales (batch, channels, blocks), blocks = ceil(h*w / 32); codes start on 16 bytes, scales on 4 (a
+ * scale is read as a byte; what matters is that both belong to one tensor of that shape).
+ */
+#define DVC_CKPT_INT8 0
+#define DVC_CKPT_E4M3 1
+typedef struct DvcCkpt {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int32_t channels;
+  int32_t format;
+} DvcCkpt;
+/* codes / scales of act(x), act = LeakyReLU(slope) when `act` (slope 0: ReLU), else the identity. */
+int dvc_act_checkpoint(const DvcSrc* x, int32_t act, float slope, int32_t format, uint8_t* codes,
+                       uint8_t* scales, int32_t batch, int32_t h, int32_t w, void* stream);
+/* out = the values the codes stand for. */
+int dvc_act_restore(const DvcCkpt* ckpt, const DvcDst* out, int32_t batch, int32_t h, int32_t w, void* stream);
+/* signs[n][c][block]: bit i = value i of the block is greater than zero (bits past the plane's end: 0). */
+int dvc_act_signs(const DvcSrc* x, uint32_t* signs, int32_t batch, int32_t h, int32_t w, void* stream);
+/* dvc_act_grad with the activation's output given by its signs (of the stored, i.e. PixelShuffle(2)-ed, tensor). */
+int dvc_act_grad_signs(const DvcSrc* grad, const uint32_t* signs, float slope, int32_t pixel_shuffle,
+                       float* grad_pre, int32_t batch, int32_t channels, int32_t ho, int32_t wo, void* stream);
+/* dvc_mul_act_grad_add with x given by its checkpoint (only the codes' sign bits are read). */
+int dvc_mul_act_grad_ckpt(const DvcSrc* grad, const DvcCkpt* x, float slope, const DvcSrc* plus, const DvcDst* out,
+                          int32_t batch, int32_t h, int32_t w, void* stream);
+/* dvc_conv2d_wgrad with the sources given by checkpoints of their activated values (all of one format).
+ * Deterministic.  The products are exact: a code times its power of two is a bf16 number, and the gradient is split
+ * into three bf16 parts that add up to it; sums are fp32.  (A block that restores to NaN, or a gradient that is not
+ * finite, reaches every weight it takes part in as NaN.) */
+int64_t dvc_conv2d_wgrad_ckpt_scratch_floats(int32_t cout, int32_t cin, int32_t ksize, int32_t stride,
+                                             int32_t batch, int32_t in_h, int32_t in_w);
+int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t batch, int32_t in_h, int32_t in_w,
+                          const float* grad_out, int32_t out_channels, int32_t ksize, int32_t stride,
+                          float* scratch, float* grad_weight, float* grad_bias, void* stream);
+
+/*
+ * ---- Log probabilities of given symbols under a distribution given class by class (the categorical counterpart of
+ * the likelihoods the reference takes from compressai's Gaussian and factorised models, dmc/train.py:74-93).
+ *
+ * Logits: class v of group g at pixel p of sample n is at ptr[n*batch_stride + (g*classes + v)*class_stride + p];
+ * class_stride >= h*w.  Symbols and all per-site results are contiguous (batch, groups, h, w).  A symbol < 0 means
+ * "none here": its log probability is 0 and has no gradient; one >= classes gives NaN.  A site whose classes are all
+ * at minus infinity has log probability -inf, entropy 0 and probabilities 0.
+ *   log_prob = log softmax(logits)[symbol], entropy = -sum p log p (nats), stats[2][sites] = (max, log of the sum of
+ *   exp(logit - max)): what dvc_symbol_log_probs_backward needs.
+ *   top (0..DVC_MAX_TOP, <= classes): the `top` most likely classes in falling order (equal logits: the lower class
+ *   first, NaN above all), as log probabilities and classes, contiguous (batch, groups * top, h, w).
+ */
+#define DVC_MAX_TOP 16
+#define DVC_F32 0
+#define DVC_BF16 1
+#define DVC_F16 2
+typedef struct DvcLogits {
+  const void* ptr;
+  int64_t batch_stride, class_stride;   /* in elements */
+  int32_t groups, classes;
+  int32_t dtype;                        /* DVC_F32 / DVC_BF16 / DVC_F16 */
+  int32_t _pad;
+} DvcLogits;
+/* scratch: dvc_symbol_log_probs_scratch_floats() floats (0: may be NULL). */
+int64_t dvc_symbol_log_probs_scratch_floats(const DvcLogits* logits, int32_t top, int32_t batch, int32_t h, int32_t w);
+int dvc_symbol_log_probs(const DvcLogits* logits, const int32_t* symbols, int32_t top, float* log_prob, float* entropy,
+                         float* stats, float* top_log_prob, int32_t* top_symbol, float* scratch, int32_t batch,
+                         int32_t h, int32_t w, void* stream);
+/* grad_logits (contiguous, the logits' type) = grad_log_prob (1[v = symbol] - p_v) - grad_entropy p_v (log p_v + entropy);
+ * grad_log_prob or grad_entropy may be NULL (zero). */
+int dvc_symbol_log_probs_backward(const DvcLogits* logits, const int32_t* symbols, const float* stats,
+                                  const float* entropy, const float* grad_log_prob, const float* grad_entropy,
+                                  void* grad_logits, int32_t batch, int32_t h, int32_t w, void* stream);
+
+/*
  * Host range coder (no GPU involved): restates compressai.ans
  * RansEncoder.encode_with_indexes / RansDecoder.decode_with_indexes as used at
  * video_model.py:238-239,250-251,257,273,283.  64-bit-state rANS, 32-bit words,

@@ -1,0 +1,479 @@
+"""8-bit activation checkpoints against the format's definition in 64 bits: codes and scales bit for bit, restored
+values, the sign-only adjoints, and weight gradients from checkpoints."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ("int8", "e4m3")
+
+
+def encode64(x, fmt):
+    """codes, scales of a CPU tensor, from the definition, in float64."""
+    n, c, h, w = x.shape
+    v = F.pad(x.double().reshape(n, c, h * w), (0, -(h * w) % 32)).view(n, c, -1, 32)
+    fine = torch.isfinite(v).all(-1, keepdim=True)
+    v0 = torch.where(fine, v, 0.0)
+    largest = 127.0 if fmt == "int8" else 448.0
+    amax = v0.abs().amax(-1, keepdim=True)
+    mant, expo = torch.frexp(amax / largest)                     # the smallest e with amax <= largest 2^e
+    e = torch.where(amax == 0, -110, torch.where(mant == 0.5, expo - 1, expo)).clamp(min=-110)
+    # amax / largest may round onto a power of two from above: settle it by an exact comparison
+    e = torch.where(amax > largest * torch.exp2(e.double()), e + 1, e)
+    y = v0.abs().clamp(max=63 * 2.0 ** 122 if fmt == "int8" else 240 * 2.0 ** 120) / torch.exp2(e.double())    # restores below 2^128
+    if fmt == "int8":
+        mag = torch.round(y)
+    else:
+        b = torch.floor(torch.log2(y.clamp(min=2.0 ** -30))).clamp(min=-6)
+        b = torch.where(torch.exp2(b) > y, (b - 1).clamp(min=-6), b)
+        q = torch.round(y / torch.exp2(b - 3))                   # in eighths of the binade (subnormals: of 2^-6)
+        mag = torch.where(b == -6, q, (b + 7) * 8 + q - 8)       # q = 16 carries into the next binade by itself
+    codes = torch.where(fine, mag, 0.0).to(torch.uint8) + (~(v > 0)).to(torch.uint8) * 128
+    scales = torch.where(fine, e + 127, 255).to(torch.uint8)
+    return codes.view(n, c, -1), scales.view(n, c, -1), fine
+
+
+def values64(codes, scales, fmt, shape):
+    n, c, h, w = shape
+    k = torch.arange(128, dtype=torch.float64)
+    mag = k if fmt == "int8" else torch.where(k < 8, k * 2.0 ** -9, (8 + k % 8) * torch.exp2(torch.floor(k / 8) - 10))
+    table = torch.cat((mag, -mag))
+    s = torch.where(scales == 255, float("nan"), torch.exp2(scales.double() - 127))
+    v = table[codes.long()].view(n, c, -1, 32) * s[..., None]
+    return v.reshape(n, c, -1)[:, :, :h * w].reshape(shape)
+
+
+def leaky32(x, slope):
+    return x if slope is None else torch.where(x > 0, x, x * torch.tensor(slope, dtype=torch.float32))
+
+
+def sample(shape, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g) * torch.exp2(6 * torch.randn(shape[:2], generator=g))[..., None, None]
+    x[torch.rand(shape, generator=g) < 0.2] = 0.0                     # as behind a ReLU
+    x[torch.rand(shape, generator=g) < 0.02] *= 2.0 ** -20            # far below their block's largest
+    return x
+
+
+SHAPES = [(1, 1, 1, 1), (1, 3, 1, 31), (2, 2, 4, 8), (1, 2, 3, 11), (2, 5, 16, 16), (1, 3, 7, 129), (3, 35, 20, 24), (1, 70, 33, 65)]
+
+
+@pytest.mark.parametrize("slope", [None, 0.0, 0.1, 1.0])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_codes_and_scales_are_those_of_the_definition(shape, fmt, slope):
+    from deepvideocodec_amd import ops
+    x = sample(shape, sum(shape))
+    ck = ops.act_checkpoint(x.cuda(), slope=slope, fmt=fmt)
+    codes, scales, _ = encode64(leaky32(x, slope), fmt)
+    assert ck.shape == shape and ck.fmt == fmt
+    assert torch.equal(ck.scales.cpu(), scales)
+    assert torch.equal(ck.codes.cpu(), codes)
+    back = ops.act_restore(ck).cpu()
+    assert torch.equal(back.double(), values64(codes, scales, fmt, shape))    # a code times a power of two is exact
+    assert torch.equal(torch.signbit(back), ~(x > 0)) or slope == 0.0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_ranges_borders_and_ties(fmt):
+    from deepvideocodec_amd import ops
+    largest = 127.0 if fmt == "int8" else 448.0
+    up = lambda v: math.ldexp(math.frexp(v)[0] + 2.0 ** -24, math.frexp(v)[1])     # the next fp32 number
+    blocks = []
+    for e in (-100, -3, 0, 5, 100):
+        blocks += [[largest * 2.0 ** e], [up(largest) * 2.0 ** e], [2.0 ** e], [1.5 * 2.0 ** e, -2.0 ** (e - 30)]]
+    # ties: halves of a step
+    blocks += [[largest] + [k + 0.5 for k in range(0, 30)], [-largest] + [-(k + 0.5) for k in range(60, 90)],
+               [largest] + [(8 + j + 0.5) * 2.0 ** s for j in range(8) for s in (-9, -5, 4)], [largest] + [(j + 0.5) * 2.0 ** -9 for j in range(9)]]
+    # smallest and largest numbers
+    blocks += [[2.0 ** -110], [2.0 ** -111, 2.0 ** -103], [1e-45], [2.0 ** -126, -1e-40], [3.4028234e38], [-3.4028234e38, 1.0], [0.0, -0.0]]
+    x = torch.zeros(len(blocks), 32)
+    for i, b in enumerate(blocks):
+        x[i, :len(b)] = torch.tensor(b)
+    x = x.view(1, len(blocks), 4, 8)
+    ck = ops.act_checkpoint(x.cuda(), fmt=fmt)
+    codes, scales, _ = encode64(x, fmt)
+    assert torch.equal(ck.scales.cpu(), scales)
+    assert torch.equal(ck.codes.cpu(), codes)
+    v = ops.act_restore(ck).cpu()
+    assert torch.equal(v.double(), values64(codes, scales, fmt, x.shape))
+    # half a step of the block's scale (int8) or of the value (e4m3: 2^-4, subnormals half of 2^-9 scale steps)
+    step = torch.exp2(scales.double() - 127).view(1, -1, 1, 1)
+    bound = step / 2 if fmt == "int8" else torch.maximum(x.double().abs() * 2.0 ** -4, step * 2.0 ** -10)
+    bound = torch.where(x.double().abs() > 1.875 * 2.0 ** 127, 2 * bound, bound)      # (rounded down, not to 2^128)
+    assert bool(((v.double() - x.double()).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_block_that_is_not_finite_restores_to_nan_and_keeps_to_itself(fmt):
+    from deepvideocodec_amd import ops
+    x = torch.randn(1, 3, 4, 32, generator=torch.Generator().manual_seed(0))
+    for row, bad in enumerate((float("inf"), float("-inf"), float("nan"))):
+        x[0, 1, row, 5 * row + 1] = bad
+    v = ops.act_restore(ops.act_checkpoint(x.cuda(), fmt=fmt)).cpu()
+    assert bool(v[0, 1, :3].isnan().all())
+    assert bool(torch.isfinite(v[0, 1, 3]).all()) and bool(torch.isfinite(v[0, 0]).all()) and bool(torch.isfinite(v[0, 2]).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_views_and_unaligned_sources(fmt):
+    """Channel slices, strided batches and planes off 16 bytes are read in place; restoring writes nothing else."""
+    from deepvideocodec_amd import ops
+    base = sample((3, 8, 6, 10), 7).cuda()
+    for view in (base[:, 2:5], base[::2], base[1:2, 3:4], base[:, 1::3], base.view(3, 8, 60, 1)[:, :, 3:43].reshape(3, 8, 40, 1)[:, 1:4]):
+        ck = ops.act_checkpoint(view, fmt=fmt)
+        codes, scales, _ = encode64(view.cpu(), fmt)
+        assert torch.equal(ck.codes.cpu(), codes) and torch.equal(ck.scales.cpu(), scales)
+        assert torch.equal(ops.act_signs(view).cpu(), signs64(view.cpu()))
+    flat = torch.zeros(4 * 63 + 1, device="cuda")
+    odd = flat[1:].view(1, 4, 7, 9)                                    # 4 bytes past an aligned address
+    odd.copy_(sample((1, 4, 7, 9), 8))
+    assert torch.equal(ops.act_checkpoint(odd, fmt=fmt).codes.cpu(), encode64(odd.cpu(), fmt)[0])
+    target = torch.full((3, 8, 6, 10), 5.0, device="cuda")
+    ck = ops.act_checkpoint(base[:, 2:5], fmt=fmt)
+    ops.act_restore(ck, out=target[:, 4:7])
+    assert torch.equal(target[:, 4:7], ops.act_restore(ck))
+    assert bool((target[:, :4] == 5).all()) and bool((target[:, 7:] == 5).all())
+
+
+def signs64(x):
+    n, c, h, w = x.shape
+    v = F.pad((x > 0).reshape(n, c, h * w), (0, -(h * w) % 32)).view(n, c, -1, 32).long()
+    return (v << torch.arange(32)).sum(-1).to(torch.int32)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_sign_only_adjoints_equal_the_fp32_ones(shape):
+    from deepvideocodec_amd import ops
+    x = sample(shape, 3 + sum(shape)).cuda()
+    g = torch.Generator().manual_seed(1)
+    grad, plus = (torch.randn(shape, generator=g).cuda() for _ in range(2))
+    signs = ops.act_signs(x)
+    assert torch.equal(signs.cpu(), signs64(x.cpu()))
+    for slope in (0.0, 0.01, 0.2):
+        assert torch.equal(ops.act_grad_signs(grad, signs, slope, False, shape), ops.act_grad(grad, x, slope, False, shape))
+        for fmt in FORMATS:
+            ck = ops.act_checkpoint(x, slope=slope, fmt=fmt)
+            assert torch.equal(ops.mul_act_grad_ckpt(grad, ck, slope), ops.mul_act_grad(grad, x, slope))
+            assert torch.equal(ops.mul_act_grad_ckpt(grad, ck, slope, plus=plus), ops.mul_act_grad(grad, x, slope, plus=plus))
+            into = grad.clone()
+            ops.mul_act_grad_ckpt(into, ck, slope, out=into)            # in place
+            assert torch.equal(into, ops.mul_act_grad(grad, x, slope))
+
+
+@pytest.mark.parametrize("n,c,h,w", [(1, 4, 1, 1), (2, 8, 5, 7), (1, 12, 8, 16)])
+def test_sign_only_adjoint_behind_a_pixel_shuffle(n, c, h, w):
+    from deepvideocodec_amd import ops
+    out = sample((n, c // 4, 2 * h, 2 * w), 5).cuda()
+    grad = torch.randn(out.shape, generator=torch.Generator().manual_seed(2)).cuda()
+    assert torch.equal(ops.act_grad_signs(grad, ops.act_signs(out), 0.1, True, (n, c, h, w)), ops.act_grad(grad, out, 0.1, True, (n, c, h, w)))
+
+
+# ---------------------------------------------------------------------------------------- weight gradients
+def wgrad64(x, g, k, stride):
+    """(gw, gb) of float64 CPU tensors, tap by tap."""
+    n, cout, ho, wo = g.shape
+    p = k // 2
+    xp = F.pad(x, (p, p, p, p))
+    gw = torch.stack([torch.stack([torch.einsum("nopq,nipq->oi", g, xp[:, :, ky:ky + (ho - 1) * stride + 1:stride, kx:kx + (wo - 1) * stride + 1:stride])
+                                   for kx in range(k)], -1) for ky in range(k)], -2)
+    return gw, g.sum((0, 2, 3))
+
+
+WGRAD = [
+    # k, stride, cins, cout, h, w, batch
+    (3, 1, (64,), 64, 36, 52, 2),
+    (3, 1, (16, 8), 40, 17, 23, 1),
+    (3, 1, (5, 7, 9, 11), 33, 21, 19, 2),
+    (3, 1, (96,), 128, 12, 20, 1),
+    (3, 1, (130,), 70, 8, 40, 1),
+    (3, 1, (48,), 48, 16, 16, 3),
+    (3, 1, (64,), 3, 9, 37, 1),
+    (3, 1, (3,), 64, 20, 28, 1),
+    (3, 1, (1,), 1, 1, 1, 1),
+    (3, 1, (2,), 5, 1, 67, 2),
+    (3, 1, (2,), 5, 67, 1, 2),
+    (3, 1, (33,), 31, 70, 66, 1),
+    (3, 2, (67,), 64, 32, 48, 1),
+    (3, 2, (16,), 24, 25, 31, 2),
+    (3, 2, (4,), 6, 1, 2, 1),
+    (3, 2, (40,), 72, 64, 130, 1),
+    (7, 1, (8,), 32, 30, 50, 1),
+    (7, 1, (16,), 2, 20, 37, 2),
+    (7, 1, (32,), 64, 19, 70, 2),
+    (7, 1, (40, 24), 16, 9, 33, 1),
+    (7, 1, (3,), 33, 2, 3, 1),
+    (1, 1, (64,), 32, 33, 47, 1),
+    (1, 1, (7, 70), 65, 1, 5, 3),
+    (1, 2, (12,), 64, 34, 50, 2),
+    (1, 2, (33,), 34, 7, 9, 1),
+]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("k,stride,cins,cout,h,w,batch", WGRAD)
+def test_weight_gradient_of_whole_numbers_is_exact(k, stride, cins, cout, h, w, batch, fmt):
+    """Whole numbers that both formats hold, small enough that every partial sum is below 2^24: no rounding happens
+    anywhere, so every layout, padding or ragged edge that is wrong by one element shows."""
+    from deepvideocodec_amd import ops
+    gen = torch.Generator().manual_seed(k + cout + h + w)
+    # 15 steps of a block's scale: exact in both formats, whatever the block's largest value is
+    xs = [torch.randint(-15, 16, (batch, c, h, w), generator=gen).float() for c in cins]
+    p = k // 2
+    ho, wo = (h + 2 * p - k) // stride + 1, (w + 2 * p - k) // stride + 1
+    g = torch.randint(-8, 9, (batch, cout, ho, wo), generator=gen).float()
+    assert batch * ho * wo * 15 * 8 < 1 << 24
+    cks = [ops.act_checkpoint(x.cuda(), fmt=fmt) for x in xs]
+    for x, ck in zip(xs, cks):
+        assert torch.equal(ops.act_restore(ck).cpu(), x)
+    gw, gb = ops.conv2d_wgrad_ckpt(cks, g.cuda(), (cout, sum(cins), k, k), stride, with_bias=True)
+    want_w, want_b = wgrad64(torch.cat(xs, 1).double(), g.double(), k, stride)
+    assert torch.equal(gw.cpu().double(), want_w)
+    assert torch.equal(gb.cpu().double(), want_b)
+    alone = ops.conv2d_wgrad_ckpt(cks, g.cuda(), (cout, sum(cins), k, k), stride)
+    assert torch.equal(alone, gw)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("k,stride,cins,cout,h,w,batch", WGRAD)
+def test_weight_gradient_of_real_numbers(k, stride, cins, cout, h, w, batch, fmt):
+    """Against 64 bits with the stored operands.  Products are exact; n terms, each in three parts, are added in fp32, so
+    a sum is off by at most 3 n 2^-24 of the sum of magnitudes (any order of addition)."""
+    from deepvideocodec_amd import ops
+    gen = torch.Generator().manual_seed(3 * k + cout + h + w)
+    xs = [sample((batch, c, h, w), 11 + c) for c in cins]
+    p = k // 2
+    ho, wo = (h + 2 * p - k) // stride + 1, (w + 2 * p - k) // stride + 1
+    g = torch.randn(batch, cout, ho, wo, generator=gen) * torch.exp2(4 * torch.randn(1, cout, 1, 1, generator=gen) - 10)
+    cks = [ops.act_checkpoint(x.cuda(), slope=0.1, fmt=fmt) for x in xs]
+    x64 = torch.cat([values64(ck.codes.cpu(), ck.scales.cpu(), fmt, ck.shape) for ck in cks], 1)
+    gw, gb = ops.conv2d_wgrad_ckpt(cks, g.cuda(), (cout, sum(cins), k, k), stride, with_bias=True)
+    want_w, want_b = wgrad64(x64, g.double(), k, stride)
+    most_w, most_b = wgrad64(x64.abs(), g.double().abs(), k, stride)
+    n = batch * ho * wo
+    assert bool(((gw.cpu().double() - want_w).abs() <= 3 * n * 2.0 ** -24 * most_w).all())
+    assert bool(((gb.cpu().double() - want_b).abs() <= n * 2.0 ** -24 * most_b).all())
+    again = ops.conv2d_wgrad_ckpt(cks, g.cuda(), (cout, sum(cins), k, k), stride, with_bias=True)
+    assert torch.equal(again[0], gw) and torch.equal(again[1], gb)       # a fixed order of addition
+
+
+def test_weight_gradient_keeps_all_bits_of_the_gradient():
+    """One pixel: the result is a single product of a 24-bit gradient and a code, correctly rounded parts and all."""
+    from deepvideocodec_amd import ops
+    gen = torch.Generator().manual_seed(5)
+    x = torch.exp2(torch.randint(-3, 4, (1, 40, 1, 1), generator=gen).float())          # powers of two: exact products
+    g = torch.randn(1, 50, 1, 1, generator=gen)
+    gw = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x.cuda()), g.cuda(), (50, 40, 1, 1))
+    assert torch.equal(gw.cpu(), g.view(50, 1, 1, 1) * x.view(1, 40, 1, 1))
+
+
+@pytest.mark.parametrize("k", [1, 3, 7])
+def test_what_is_not_finite_reaches_the_weights_it_takes_part_in(k):
+    from deepvideocodec_amd import ops
+    gen = torch.Generator().manual_seed(6)
+    x, g = torch.randn(1, 40, 20, 40, generator=gen), torch.randn(1, 36, 20, 40, generator=gen)
+    x[0, 7, 10, 20] = float("inf")
+    gw = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x.cuda()), g.cuda(), (36, 40, k, k)).cpu()
+    assert bool(gw[:, 7].isnan().all()) and bool(torch.isfinite(gw[:, :7]).all()) and bool(torch.isfinite(gw[:, 8:]).all())
+    x[0, 7, 10, 20] = 0.0
+    for bad in (float("nan"), float("inf")):
+        g[0, 5, 3, 4] = bad
+        gw, gb = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x.cuda()), g.cuda(), (36, 40, k, k), with_bias=True)
+        gw, gb = gw.cpu(), gb.cpu()
+        assert not bool(torch.isfinite(gw[5]).any()) and not bool(torch.isfinite(gb[5]))
+        assert bool(torch.isfinite(gw[:5]).all()) and bool(torch.isfinite(gw[6:]).all()) and bool(torch.isfinite(gb[6:]).all())
+
+
+def test_refusals_of_the_python_surface():
+    from deepvideocodec_amd import ops
+    x = torch.randn(2, 4, 8, 8, device="cuda")
+    ck = ops.act_checkpoint(x)
+    with pytest.raises(ValueError, match="slope"):
+        ops.act_checkpoint(x, slope=1.5)
+    with pytest.raises(ValueError, match="slope"):
+        ops.act_checkpoint(x, slope=-0.5)
+    with pytest.raises(TypeError):
+        ops.act_checkpoint(x.half())
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.act_checkpoint(x.transpose(2, 3)[:, :, :, ::2])
+    with pytest.raises(ValueError, match="elements"):
+        ops.act_restore(ck._replace(codes=ck.codes[:1].contiguous()))
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.act_restore(ck._replace(codes=ck.codes.transpose(0, 1)))
+    with pytest.raises(ValueError, match="shape"):
+        ops.act_restore(ck, out=torch.empty(2, 4, 8, 9, device="cuda"))
+    g = torch.randn(2, 6, 8, 8, device="cuda")
+    with pytest.raises(ValueError, match="grad_pre"):
+        ops.conv2d_wgrad_ckpt(ck, g, (6, 4, 3, 3), 2)
+    with pytest.raises(ValueError, match="weight shape"):
+        ops.conv2d_wgrad_ckpt(ck, g, (6, 5, 3, 3))
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.conv2d_wgrad_ckpt(ck, g.transpose(2, 3), (6, 4, 3, 3))
+    with pytest.raises(ValueError, match="match"):
+        ops.conv2d_wgrad_ckpt((ck, ops.act_checkpoint(x, fmt="e4m3")), g, (6, 8, 3, 3))
+    with pytest.raises(_lib_error(), match="ksize"):
+        ops.conv2d_wgrad_ckpt(ck, g, (6, 4, 5, 5))
+    with pytest.raises(ValueError, match="elements"):
+        ops.act_grad_signs(g, ops.act_signs(x), 0.1, False, tuple(g.shape))
+    with pytest.raises(ValueError, match="shape"):
+        ops.mul_act_grad_ckpt(g, ck, 0.1)
+
+
+def _lib_error():
+    from deepvideocodec_amd import _lib
+    return _lib.DvcError
+
+
+def test_on_a_side_stream_and_in_a_replayed_graph():
+    from deepvideocodec_amd import ops
+    gen = torch.Generator().manual_seed(9)
+    x = torch.randn(2, 40, 24, 40, generator=gen).cuda()
+    g = torch.randn(2, 48, 24, 40, generator=gen).cuda()
+
+    def passes():
+        ck = ops.act_checkpoint(x, slope=0.1)
+        gp = ops.act_grad_signs(g, ops.act_signs(g), 0.1, False, tuple(g.shape))
+        return ops.conv2d_wgrad_ckpt(ck, gp, (48, 40, 3, 3), with_bias=True) + (ops.mul_act_grad_ckpt(x, ck, 0.1),)
+
+    want = [t.clone() for t in passes()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = passes()
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = passes()
+    for round_ in range(4):
+        x.copy_(torch.randn(x.shape, generator=gen))
+        g.copy_(torch.randn(g.shape, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, passes()):
+            assert torch.equal(a, b), round_
+
+
+# ---------------------------------------------------------------------------------------- on the tape
+CONV = [
+    # k, stride, cins, cout, H, W, batch, in_slope, out_slope, shuffle
+    (3, 1, (64,), 64, 36, 52, 2, None, None, False),
+    (3, 1, (16, 8), 40, 17, 23, 1, 0.1, 0.01, False),
+    (3, 2, (67,), 64, 32, 48, 1, None, 0.1, False),
+    (7, 1, (16,), 2, 20, 37, 2, None, 0.0, False),
+    (1, 1, (32,), 8, 9, 11, 1, 0.0, None, True),
+    (3, 1, (24,), 32, 10, 14, 2, None, 0.01, True),
+]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("k,stride,cins,cout,H,W,batch,in_slope,out_slope,shuffle", CONV)
+def test_convolution_on_the_tape(k, stride, cins, cout, H, W, batch, in_slope, out_slope, shuffle, fmt):
+    """With 8-bit storage outputs, data gradients and bias gradients keep their bits; the weight gradient is that of the
+    restored operands."""
+    from deepvideocodec_amd import autograd as A, ops
+    gen = torch.Generator().manual_seed(k + cout + H)
+    xs = [torch.randn(batch, c, H, W, generator=gen).cuda().requires_grad_() for c in cins]
+    wt = (torch.randn(cout, sum(cins), k, k, generator=gen) / math.sqrt(sum(cins) * k * k)).cuda().requires_grad_()
+    b = torch.randn(cout, generator=gen).cuda().requires_grad_()
+    res = {}
+    for storage in (None, fmt):
+        y = A.conv2d(xs, wt, b, stride=stride, in_slope=in_slope, out_slope=out_slope, pixel_shuffle=shuffle, storage=storage)
+        R = torch.randn(y.shape, generator=torch.Generator().manual_seed(1)).cuda()
+        res[storage] = (y.detach(),) + torch.autograd.grad(y, [*xs, wt, b], R)
+    n = len(xs)
+    for a, c in zip(res[None][:1 + n], res[fmt][:1 + n]):
+        assert torch.equal(a, c)
+    cks = [ops.act_checkpoint(x.detach(), in_slope, fmt) for x in xs]
+    p = k // 2
+    ho, wo = (H + 2 * p - k) // stride + 1, (W + 2 * p - k) // stride + 1
+    g = R if out_slope is None and not shuffle else ops.act_grad(R, res[None][0], 1.0 if out_slope is None else out_slope, shuffle, (batch, cout, ho, wo))
+    x64 = torch.cat([ops.act_restore(ck).cpu().double() for ck in cks], 1)
+    want, want_b = wgrad64(x64, g.cpu().double(), k, stride)
+    most, most_b = wgrad64(x64.abs(), g.cpu().double().abs(), k, stride)
+    pixels = batch * ho * wo
+    assert bool(((res[fmt][1 + n].cpu().double() - want).abs() <= 3 * pixels * 2.0 ** -24 * most).all())
+    assert bool(((res[fmt][2 + n].cpu().double() - want_b).abs() <= pixels * 2.0 ** -24 * most_b).all())
+    # and no further from the weight gradient of the operands themselves than the storage's rounding takes it
+    x32 = torch.cat([leaky32(x.detach().cpu(), in_slope) for x in xs], 1).double()
+    off = wgrad64((x64 - x32).abs(), g.cpu().double().abs(), k, stride)[0]
+    ref, most_ref = res[None][1 + n].cpu().double(), wgrad64(x32.abs(), g.cpu().double().abs(), k, stride)[0]
+    assert bool(((res[fmt][1 + n].cpu().double() - ref).abs() <= off + 3 * pixels * 2.0 ** -24 * (most + 2 * most_ref)).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kw", [dict(slope=0.01), dict(slope=0.0), dict(slope=0.1, start_from_relu=True, end_with_relu=True, bottleneck=True),
+                                dict(slope=0.01, start_from_relu=False)])
+def test_residual_block_on_the_tape(kw, fmt):
+    """Outputs and data gradients keep their bits; the weight and bias gradients are those of the same two convolutions
+    taken one by one with the same storage."""
+    from deepvideocodec_amd import autograd as A
+    from deepvideocodec_amd.models.layers import ResBlock
+    torch.manual_seed(0)
+    blk = ResBlock(32, **kw).cuda()
+    x = torch.randn(2, 32, 18, 26).cuda().requires_grad_()
+    plus = torch.randn(2, 32, 18, 26).cuda().requires_grad_()
+    R = torch.randn(2, 32, 18, 26).cuda()
+    params = [blk.conv1.weight, blk.conv1.bias, blk.conv2.weight, blk.conv2.bias]
+    res = {}
+    for storage in (None, fmt):
+        blk.conv1.act_storage = blk.conv2.act_storage = storage
+        y = blk(x, plus=plus)
+        res[storage] = (y.detach(),) + torch.autograd.grad(y, [x, plus, *params], R)
+    for i in (0, 1, 2):
+        assert torch.equal(res[None][i], res[fmt][i]), i
+    s_in, s_mid, s_out = blk.slope if blk.start_from_relu else None, blk.slope, blk.slope if blk.end_with_relu else None
+    t = A.conv2d(x, blk.conv1.weight, blk.conv1.bias, in_slope=s_in, out_slope=s_mid, storage=fmt)
+    y = A.conv2d(t, blk.conv2.weight, blk.conv2.bias, out_slope=s_out, residual=x, residual2=plus, storage=fmt)
+    for a, c in zip(torch.autograd.grad(y, params, R), res[fmt][3:]):
+        assert torch.equal(a, c)
+
+
+def test_squeeze_excite_pieces_on_the_tape():
+    from deepvideocodec_amd import autograd as A, ops
+    torch.manual_seed(0)
+    a, b, g = (torch.randn(2, 32, 20, 24).cuda() for _ in range(3))
+    scale = torch.rand(64).cuda().requires_grad_()
+    fc1, fc2 = torch.randn(4, 32).cuda().requires_grad_(), torch.randn(32, 4).cuda().requires_grad_()
+    b.requires_grad_()
+    for storage in ("int8", "e4m3"):
+        gb, gs = torch.autograd.grad(A.add_scaled(a, b, scale, storage=storage), [b, scale], g)
+        assert torch.equal(gb, torch.autograd.grad(A.add_scaled(a, b, scale), b, g)[0])
+        stored = ops.act_restore(ops.act_checkpoint(b.detach(), fmt=storage))
+        assert torch.equal(gs, ops.plane_dot(g, stored).view_as(gs))
+        r = torch.randn(64).cuda()
+        for u, v in zip(torch.autograd.grad(A.se_gate(b, fc1, fc2, storage), [b, fc1, fc2], r), torch.autograd.grad(A.se_gate(b, fc1, fc2), [b, fc1, fc2], r)):
+            assert torch.equal(u, v)
+
+
+def test_training_step_on_8_bit_storage(seeded_sd):
+    """The model's own training step with 8-bit storage: the same loss to the bit, gradients for the same parameters, less
+    memory held by the tape.  (The layers' gradients are held to the definition above, layer by layer.)"""
+    from deepvideocodec_amd import train as TR
+    from deepvideocodec_amd.models import DMC
+    from deepvideocodec_amd.testing import synthetic_gop
+    frames = [f.cuda() for f in synthetic_gop(3, 128, 128, seed=3, batch=2)]
+    res, held = {}, {}
+    for storage in ("fp32", "int8", "e4m3"):
+        net = DMC()
+        net.load_state_dict(seeded_sd)
+        net = net.cuda().train().set_act_storage(storage)
+        torch.manual_seed(5)
+        net(list(frames))                     # (weight images are built on first use and kept)
+        torch.manual_seed(5)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = TR.RateDistortionLoss(lmbda=2048.0)(net(list(frames)), frames[1:])
+        held[storage] = torch.cuda.memory_allocated() - before
+        out["loss"].backward()
+        res[storage] = (out["loss"].item(), {n: p.grad for n, p in net.named_parameters() if p.grad is not None})
+        del net, out
+    for storage in ("int8", "e4m3"):
+        assert res[storage][0] == res["fp32"][0]
+        assert set(res[storage][1]) == set(res["fp32"][1])
+        assert all(bool(torch.isfinite(g).all()) for g in res[storage][1].values())
+        assert held[storage] < held["fp32"], held

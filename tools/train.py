@@ -86,6 +86,8 @@ def main(argv=None):
     ap.add_argument("--save", default=None, help="directory for checkpoint.pth.tar / checkpoint_best_loss.pth.tar")
     ap.add_argument("--checkpoint", default=None)
     ap.add_argument("--seed", type=int, default=None)
+    ap.add_argument("--act-storage", default="fp32", help="what the tape keeps of the convolutions' operands: fp32, or 8-bit "
+                                                          "checkpoints (int8, e4m3)")
     args = ap.parse_args(argv)
 
     rank = int(os.environ.get("RANK", "0"))
@@ -118,6 +120,7 @@ def main(argv=None):
     test_loader = torch.utils.data.DataLoader(test_ds, batch_size=args.test_batch_size, num_workers=args.num_workers,
                                               shuffle=False, sampler=sampler(test_ds, False), pin_memory=True)
     net = DMC().to(dev)           # Xavier-normal initial weights, like the reference's constructor
+    net.set_act_storage(args.act_storage)
     if world > 1:                 # same initial weights on every rank
         import torch.distributed as dist
         for t in list(net.parameters()) + list(net.buffers()):

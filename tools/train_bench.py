@@ -28,6 +28,8 @@ def main():
     ap.add_argument("--recompute", type=int, default=0, help="1: recompute the reconstruction / fusion blocks in backward")
     ap.add_argument("--precision", default="fp32", help="operand mode of the forward / data-gradient convolutions "
                                                         "(fp32, fp16x2, bf16x2, bf16); weight gradients stay fp32")
+    ap.add_argument("--act-storage", default="fp32", help="what the tape keeps of the convolutions' operands: fp32, or 8-bit "
+                                                          "checkpoints (int8, e4m3)")
     ap.add_argument("--gpus", type=int, default=None,
                     help="ranks (one process per GPU); N > 1 without a launcher starts torch.distributed.run itself")
     args = ap.parse_args()
@@ -47,6 +49,7 @@ def main():
     net = net.to(dev).train()
     net.recompute = bool(args.recompute)
     net.set_precision(args.precision, train=True)
+    net.set_act_storage(args.act_storage)
     crit = TR.RateDistortionLoss(lmbda=2048.0)
     opt, aux_opt = TR.configure_optimizers(net, 1e-4, 1e-3)
     batches = [[f.to(dev) for f in synthetic_gop(args.frames, args.size, args.size, seed=rank * 100 + s, batch=args.batch)]
@@ -81,7 +84,7 @@ def main():
             "value": args.batch * world * args.steps / el, "unit": "samples/s", "n_gpus": world, "world_size": world,
             "steps": args.steps,
             "warmup": args.warmup, "ms_per_step": el / args.steps * 1e3, "batch_per_gpu": args.batch,
-            "recompute": bool(args.recompute),
+            "recompute": bool(args.recompute), "act_storage": args.act_storage,
             "approx_tflops_per_gpu": 3 * fwd_tflop / (el / args.steps), "last_step": stats,
             "max_mem_gb": torch.cuda.max_memory_allocated() / 2 ** 30,
             "dtype": "f32" if args.precision == "fp32" else "f32 (%s operands in the forward / data-gradient convolutions)" % args.precision,
