@@ -90,7 +90,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(unsigned long long at, un
 
 struct __attribute__((packed)) Dword { unsigned v; };      // a dword at any byte address
 
-__device__ __forceinline__ float scale_of(unsigned s) { return s == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(s << 23); }
+__device__ __forceinline__ float scale_of(unsigned s, unsigned flip) { return __uint_as_float((s == 255u ? 0x7fc00000u : s << 23) ^ flip); }
 
 // four codes -> two dwords of bf16 (exact); s01 / s23 ... one scale per code
 template <bool E4M3>
@@ -105,8 +105,8 @@ __device__ __forceinline__ uint2 decode(unsigned k, float s0, float s1, float s2
     const unsigned m = k & 0x7f7f7f7fu, sg = k & 0x80808080u;
     const float f0 = (float)(m & 0xffu) * s0, f1 = (float)((m >> 8) & 0xffu) * s1;
     const float f2 = (float)((m >> 16) & 0xffu) * s2, f3 = (float)(m >> 24) * s3;
-    r.x = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u) | __builtin_amdgcn_perm(0u, sg, 0x010c000cu);
-    r.y = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u) | __builtin_amdgcn_perm(0u, sg, 0x030c020cu);
+    r.x = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u) ^ __builtin_amdgcn_perm(0u, sg, 0x010c000cu);
+    r.y = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u) ^ __builtin_amdgcn_perm(0u, sg, 0x030c020cu);
   }
   return r;
 }
@@ -196,6 +196,11 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
   const unsigned plane_bytes = 32u * (unsigned)a.blocks;
   const unsigned gplane = (unsigned)(a.ho * a.wo);
 
+  // Every second slab is computed with its inputs' signs changed and changed back when it is stored: the matrix
+  // instruction cuts what lies far below its running sum downwards, and over the slabs that drift cancels (64->64 3x3 at
+  // 32x256x256: relative error 2.0e-6 without, of which 93 % is drift).  It costs nothing: the sign rides on the scale.
+  const unsigned flip = (blockIdx.x & 1u) << 31;
+
   Plane xp[XPW];
 #pragma unroll
   for (int c = 0; c < XPW; ++c) xp[c] = plane_of(a, ci0 + XPW * wave + c);
@@ -217,7 +222,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
   int cut[XSLOTS];              // codes of a dword before a block's end (not AL)
   float4 gr[GLOADS];
 
-  auto load = [&](int t) {      // request tile t (past the last: zeros)
+  auto load = [&](int t) __attribute__((always_inline)) {      // request tile t (past the last: zeros)
     const bool there = t < a.n_tiles;
     const int tt = there ? t : 0;
     const int n = tt / per_n, r = tt - n * per_n;
@@ -280,18 +285,18 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     }
   };
 
-  auto store_as = [&](char* buf, auto e4m3) {      // decode what load() requested into an LDS buffer
+  auto store_as = [&](char* buf, auto e4m3) __attribute__((always_inline)) {      // decode what load() requested into an LDS buffer
 #pragma unroll
     for (int j = 0; j < XSLOTS; ++j) {
       const int e = lane + 64 * j, iy = e / G::XD, q = e - iy * G::XD;
 #pragma unroll
       for (int c = 0; c < XPW; ++c) {
-        const float s0 = scale_of(xs[c][j]);
+        const float s0 = scale_of(xs[c][j], flip);
         uint2 v;
         if constexpr (AL) {
           v = decode<decltype(e4m3)::value>(xk[c][j], s0, s0, s0, s0);
         } else {
-          const float s4 = scale_of(xs2[c][j]);
+          const float s4 = scale_of(xs2[c][j], flip);
           v = decode<decltype(e4m3)::value>(xk[c][j], s0, cut[j] > 1 ? s0 : s4, cut[j] > 2 ? s0 : s4, cut[j] > 3 ? s0 : s4);
           // codes past the row's end are padding: zeros (also where the scale is that of a poisoned block)
           v.x = mask[j] > 1 ? v.x : mask[j] > 0 ? v.x & 0xffffu : 0u;
@@ -321,7 +326,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     }
   };
 
-  auto store = [&](char* buf) {
+  auto store = [&](char* buf) __attribute__((always_inline)) {
     if (a.e4m3) store_as(buf, std::true_type{});
     else store_as(buf, std::false_type{});
   };
@@ -335,7 +340,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
   const int ga = G::XBYTES + (mt * 32 + l32) * G::GUNITS * 16 + half * 32;
   const int xa = (ct * 32 + l32) * G::XUNITS * 16 + half * 16;
 
-  auto multiply = [&](const char* buf, int step) {       // one row piece
+  auto multiply = [&](const char* buf, int step) __attribute__((always_inline)) {       // one row piece
     const int row = step / (TW / 16), px = step % (TW / 16) * 16;
     const float4* const gp = reinterpret_cast<const float4*>(buf + ga + (row * TW + px) * 4);
     const Split s = split(gp[0], gp[1]);
@@ -371,18 +376,27 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     }
   };
 
+  // Of the two waves of a SIMD one stages before it multiplies and one after: between the same two barriers the decoding
+  // of the one runs beside the matrix instructions of the other.
+  const bool late = wave >= 4;
   int t = blockIdx.x, b = 0;
   load(t);
   store(lds);
   load(t + nsplit);
   __syncthreads();
   for (; t < a.n_tiles; t += nsplit) {
-    store(lds + (b ^ 1) * G::BUF);          // tile t + nsplit (zeros past the last)
-    load(t + 2 * nsplit);
     const char* const buf = lds + b * G::BUF;
+    if (!late) {
+      store(lds + (b ^ 1) * G::BUF);        // tile t + nsplit (zeros past the last)
+      load(t + 2 * nsplit);
+    }
     if (KS != 7 || wave < 7) {
 #pragma unroll
       for (int i = 0; i < G::STEPS / KG; ++i) multiply(buf, i * KG + grp);
+    }
+    if (late) {
+      store(lds + (b ^ 1) * G::BUF);
+      load(t + 2 * nsplit);
     }
     __syncthreads();
     b ^= 1;
@@ -414,6 +428,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
 
   // add the waves of a corner, tap by tap; register r of a tile is row (r & 3) + 8 (r >> 2) + 4 half, column l32
   float* const red = reinterpret_cast<float*>(lds);
+  auto unflip = [&](float v) { return __uint_as_float(__float_as_uint(v) ^ flip); };
   float* const pbase = a.partial + (long long)blockIdx.x * TAPS * a.cout_pad * a.cin_pad;
   if constexpr (KS == 7) {
     if (wave < 7) {
@@ -421,7 +436,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
       for (int kx = 0; kx < 7; ++kx) {
         float* const pt = pbase + (long long)(wave * 7 + kx) * a.cout_pad * a.cin_pad + ci0 + l32;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) pt[(long long)(co0 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = acc[kx][r];
+        for (int r = 0; r < 16; ++r) pt[(long long)(co0 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = unflip(acc[kx][r]);
       }
     }
     return;
@@ -444,7 +459,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
       }
       float* const pt = pbase + (long long)tp * a.cout_pad * a.cin_pad + ci0 + ct * 32 + l32;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) pt[(long long)(co0 + mt * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = v[r];
+      for (int r = 0; r < 16; ++r) pt[(long long)(co0 + mt * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = unflip(v[r]);
     }
     if (KG > 1) __syncthreads();
   }
