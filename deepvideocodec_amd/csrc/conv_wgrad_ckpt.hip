@@ -9,10 +9,13 @@ int launch_aligned(int ks, int stride, const Args& a, const Plan& p, hipStream_t
 namespace {
 
 // gW[co][ci][tap] = sum over splits of partial[split][tap][co][ci], gB[co] likewise (indices past the weight's).  A block
-// takes 64 results; each of its waves adds every fourth split, the four sums are added in a fixed order.
-__global__ __launch_bounds__(256) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int nsplit, int taps, int cout, int cin,
-                                                                int cout_pad, int cin_pad, const float* bias_partial, float* gb) {
-  __shared__ float part[4][64];
+// takes 64 results; each of its WAVES waves adds every WAVES-th split, with the loads of four splits in flight, and the sums
+// are added in a fixed order.  16 waves for many splits (256 of a 64 x 64 3x3 layer: 9 us, 20 with four waves and one load
+// after the other), 4 for few.
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int nsplit, int taps, int cout, int cin,
+                                                                 int cout_pad, int cin_pad, const float* bias_partial, float* gb) {
+  __shared__ float part[WAVES][64];
   const long long total = (long long)cout * taps * cin;
   const long long total_all = total + (gb != nullptr ? cout : 0);
   const int lane = threadIdx.x & 63, kg = threadIdx.x >> 6;
@@ -21,9 +24,8 @@ __global__ __launch_bounds__(256) void wgrad_ckpt_reduce_kernel(const float* par
     const float* p = nullptr;
     long long step = 0, dst = -1;
     if (i < total) {
-      const int ci = (int)(i % cin);
-      const long long q = i / cin;
-      const int tap = (int)(q % taps), co = (int)(q / taps);
+      const unsigned r = (unsigned)i, ci = r % (unsigned)cin, q = r / (unsigned)cin;      // (a weight has below 2^31 elements)
+      const unsigned tap = q % (unsigned)taps, co = q / (unsigned)taps;
       p = partial + ((long long)tap * cout_pad + co) * cin_pad + ci;
       step = (long long)taps * cout_pad * cin_pad;
       dst = ((long long)co * cin + ci) * taps + tap;
@@ -32,12 +34,20 @@ __global__ __launch_bounds__(256) void wgrad_ckpt_reduce_kernel(const float* par
       step = cout_pad;
     }
     float s = 0.f;
-    if (p != nullptr)
-      for (int k = kg; k < nsplit; k += 4) s += p[k * step];
+    if (p != nullptr) {
+      int k = kg;
+      for (; k + 3 * WAVES < nsplit; k += 4 * WAVES) {
+        const float v0 = p[k * step], v1 = p[(k + WAVES) * step], v2 = p[(k + 2 * WAVES) * step], v3 = p[(k + 3 * WAVES) * step];
+        s += (v0 + v1) + (v2 + v3);
+      }
+      for (; k < nsplit; k += WAVES) s += p[k * step];
+    }
     part[kg][lane] = s;
     __syncthreads();
     if (kg == 0 && p != nullptr) {
-      const float v = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+      float v = part[0][lane];
+#pragma unroll
+      for (int k = 1; k < WAVES; ++k) v += part[k][lane];
       if (dst >= 0) gw[dst] = v;
       else gb[i - total] = v;
     }
@@ -51,6 +61,7 @@ int make_plan(int cout, int cin, int ks, int stride, int batch, int h, int w, Pl
   DVC_REQUIRE(!(ks == 7 && stride != 1), "%s: 7x7 stride 2 unsupported", who);
   DVC_REQUIRE(cout >= 1 && cin >= 1 && batch >= 1 && h >= 1 && w >= 1, "%s: bad dims", who);
   DVC_REQUIRE((long long)h * w < (1LL << 28), "%s: plane too large", who);
+  DVC_REQUIRE(((long long)h * w + 31) / 32 * cin < (1LL << 31) && (long long)cout * cin * ks * ks < (1LL << 31), "%s: too many channels", who);
   const int pad = ks / 2;
   p->ho = (h + 2 * pad - ks) / stride + 1;
   p->wo = (w + 2 * pad - ks) / stride + 1;
@@ -155,10 +166,15 @@ extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t
   a.tiles_y = p.tiles_y;
   a.n_tiles = p.n_tiles;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool aligned = in_w % 4 == 0 && p.wo % 4 == 0 && reinterpret_cast<uintptr_t>(grad_out) % 16 == 0;
+  const bool aligned = in_w % 4 == 0 && p.wo % 4 == 0 && reinterpret_cast<uintptr_t>(grad_out) % 16 == 0 &&
+                       4LL * out_channels * p.ho * p.wo < (1LL << 31);
   if (int rc = aligned ? launch_aligned(ksize, stride, a, p, st) : launch_any(ksize, stride, a, p, st)) return rc;
   const long long total = (long long)out_channels * cin * p.taps + out_channels;
-  hipLaunchKernelGGL(wgrad_ckpt_reduce_kernel, dim3(dvc::stream_grid(total, 64)), dim3(256), 0, st, scratch, grad_weight, p.nsplit,
-                     p.taps, out_channels, cin, p.cout_pad, p.cin_pad, a.bias_partial, grad_bias);
+  const dim3 grid((unsigned)((total + 63) / 64 < 16384 ? (total + 63) / 64 : 16384));
+#define REDUCE(WAVES) hipLaunchKernelGGL(wgrad_ckpt_reduce_kernel<WAVES>, grid, dim3(64 * WAVES), 0, st, scratch, grad_weight, p.nsplit, \
+                                         p.taps, out_channels, cin, p.cout_pad, p.cin_pad, a.bias_partial, grad_bias)
+  if (p.nsplit >= 64) REDUCE(16);
+  else REDUCE(4);
+#undef REDUCE
   return dvc::check_launch("wgrad_ckpt_reduce_kernel");
 }

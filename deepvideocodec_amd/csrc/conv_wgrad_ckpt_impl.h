@@ -53,12 +53,10 @@ __device__ __forceinline__ unsigned long long uniform64(unsigned long long v) {
   return ((unsigned long long)hi << 32) | lo;
 }
 
-// Where input channel `ci` (uniform) of the concatenated checkpoints lives: its plane's blocks in sample 0 counted from the
-// source's first, and the blocks between samples.  Channels past the last: live = 0.
+// Where input channel `ci` (uniform) of the concatenated checkpoints lives.
 struct Plane {
   unsigned long long codes, scales;      // addresses of sample 0's plane
-  unsigned long long step;               // blocks between samples
-  unsigned live;                         // all-ones or zero
+  unsigned step;                         // blocks between samples (< 2^31: checked on the host)
 };
 __device__ __forceinline__ Plane plane_of(const Args& a, int ci) {
   // (mask arithmetic instead of indexing by a run-time source number, which would become a private lookup table)
@@ -74,13 +72,12 @@ __device__ __forceinline__ Plane plane_of(const Args& a, int ci) {
                                     (unsigned long long)a.scales[2], (unsigned long long)a.scales[3]);
   const unsigned long long first = pick(a.first[0], a.first[1], a.first[2], a.first[3]);
   const unsigned long long chans = pick(a.chans[0], a.chans[1], a.chans[2], a.chans[3]);
-  const bool have = ci < a.cin;
+  const bool have = ci < a.cin;         // (channels past the last: any plane; their loads are switched off)
   const unsigned long long at = have ? ((unsigned long long)ci - first) * (unsigned)a.blocks : 0ull;
   Plane p;
   p.codes = uniform64((have ? c : (unsigned long long)a.codes[0]) + 32ull * at);
   p.scales = uniform64((have ? s : (unsigned long long)a.scales[0]) + at);
-  p.step = uniform64(have ? chans * (unsigned)a.blocks : 0ull);
-  p.live = __builtin_amdgcn_readfirstlane(have ? 0xffffffffu : 0u);
+  p.step = __builtin_amdgcn_readfirstlane(have ? (unsigned)(chans * (unsigned)a.blocks) : 0u);
   return p;
 }
 
@@ -204,9 +201,11 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
   Plane xp[XPW];
 #pragma unroll
   for (int c = 0; c < XPW; ++c) xp[c] = plane_of(a, ci0 + XPW * wave + c);
+  const int xlive = a.cin - (ci0 + XPW * wave);      // this wave's channels that exist
   // gradient units: unit u = tid + 512 i is unit u % GE of channel u / GE
-  unsigned gsrc[GLOADS];        // this lane's channel, as an offset in planes; past the last channel: none
+  unsigned gsrc[GLOADS];        // this lane's channel; past the last: none
   int gdst[GLOADS];
+  const unsigned gsample = 4u * (unsigned)a.cout * gplane;      // AL: below 2^31 (checked on the host)
 #pragma unroll
   for (int i = 0; i < GLOADS; ++i) {
     const int u = tid + 512 * i, ch = u / G::GE, e = u - ch * G::GE;
@@ -244,7 +243,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
 #pragma unroll
     for (int c = 0; c < XPW; ++c) {
       const unsigned long long b = (unsigned long long)(unsigned)n * xp[c].step;
-      const unsigned live = there ? xp[c].live : 0u;
+      const unsigned live = there && c < xlive ? 0xffffffffu : 0u;
 #pragma unroll
       for (int j = 0; j < XSLOTS; ++j) {
         if constexpr (AL) {
@@ -267,15 +266,17 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     // gradients: four adjacent pixels of a row
 #pragma unroll
     for (int i = 0; i < GLOADS; ++i) {
-      const int u = tid + 512 * i, e = u % G::GE;
+      const int e = (tid + 512 * i) % G::GE;
       const int oy = oy0 + 4 * e / TW, ox = ox0 + 4 * e % TW;
-      const bool ok = there && gsrc[i] != 0xffffffffu && oy < a.ho && ox < a.wo;
-      const float* const p = a.g + ((unsigned long long)(unsigned)n * a.cout + (ok ? gsrc[i] : 0u)) * gplane + (ok ? oy * a.wo + ox : 0);
-      gr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (ok) {
-        if constexpr (AL) {
-          gr[i] = *reinterpret_cast<const float4*>(p);
-        } else {
+      const bool ok = gsrc[i] != 0xffffffffu && oy < a.ho && ox < a.wo;
+      if constexpr (AL) {
+        const unsigned at = ok ? 4u * (gsrc[i] * gplane + (unsigned)(oy * a.wo + ox)) : 0x80000000u;
+        gr[i] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(
+            rsrc((unsigned long long)a.g + (unsigned long long)(unsigned)n * gsample, there ? gsample : 0u), at, 0, 0));
+      } else {
+        const float* const p = a.g + ((unsigned long long)(unsigned)n * a.cout + (ok ? gsrc[i] : 0u)) * gplane + (ok ? oy * a.wo + ox : 0);
+        gr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ok && there) {
           gr[i].x = p[0];
           if (ox + 1 < a.wo) gr[i].y = p[1];
           if (ox + 2 < a.wo) gr[i].z = p[2];
@@ -379,27 +380,26 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
   // Of the two waves of a SIMD one stages before it multiplies and one after: between the same two barriers the decoding
   // of the one runs beside the matrix instructions of the other.
   const bool late = wave >= 4;
-  int t = blockIdx.x, b = 0;
+  int t = blockIdx.x, buf = 0;
   load(t);
   store(lds);
   load(t + nsplit);
   __syncthreads();
   for (; t < a.n_tiles; t += nsplit) {
-    const char* const buf = lds + b * G::BUF;
     if (!late) {
-      store(lds + (b ^ 1) * G::BUF);        // tile t + nsplit (zeros past the last)
+      store(lds + (G::BUF - buf));        // tile t + nsplit (zeros past the last)
       load(t + 2 * nsplit);
     }
     if (KS != 7 || wave < 7) {
 #pragma unroll
-      for (int i = 0; i < G::STEPS / KG; ++i) multiply(buf, i * KG + grp);
+      for (int i = 0; i < G::STEPS / KG; ++i) multiply(lds + buf, i * KG + grp);
     }
     if (late) {
-      store(lds + (b ^ 1) * G::BUF);
+      store(lds + (G::BUF - buf));
       load(t + 2 * nsplit);
     }
     __syncthreads();
-    b ^= 1;
+    buf = G::BUF - buf;
   }
 
   // bias gradient: the lanes of a channel are GE adjacent ones (a multiple of 32): butterfly within 32, then one atomic-free

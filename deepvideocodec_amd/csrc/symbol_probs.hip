@@ -81,6 +81,10 @@ __device__ __forceinline__ float given(const typename Elem<DT>::type* row, long 
   return log_p(Elem<DT>::up(row[sym * cs]), m, log_s);
 }
 
+__device__ __forceinline__ float given_log_p(int sym, int classes, float x, float m, float log_s) {
+  return sym < 0 ? 0.f : sym >= classes ? __uint_as_float(0x7fc00000u) : log_p(x, m, log_s);
+}
+
 // order of the alternatives: larger logit first, NaN above all, then the lower class.  +0 and -0 are equal.
 __device__ __forceinline__ unsigned order_key(float x) {
   const unsigned b = __float_as_uint(x + 0.f);
@@ -101,6 +105,19 @@ __device__ __forceinline__ unsigned wave_max(unsigned v) {    // uniform result
   const unsigned c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
   const unsigned ab = a > b ? a : b, cd = c > d ? c : d;
   return ab > cd ? ab : cd;
+}
+
+// Lanes 0..15 hold a value each (others: anything): the `nth` largest of the sixteen, uniform.  A value has at least `nth`
+// not smaller than itself exactly if it is at most the nth largest.
+template <int R>
+__device__ __forceinline__ int not_below(unsigned v) {
+  const unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x120 + R, 0xF, 0xF, true);      // row_ror R
+  if constexpr (R > 1) return (o >= v ? 1 : 0) + not_below<R - 1>(v);
+  else return o >= v ? 1 : 0;
+}
+__device__ __forceinline__ unsigned nth_of_16(unsigned v, int nth, int lane) {
+  const int ge = 1 + not_below<15>(v);
+  return wave_max(lane < 16 && ge >= nth ? v : 0);
 }
 
 __device__ __forceinline__ void wave_join(Stat* st) {
@@ -140,15 +157,41 @@ struct WaveList {
   }
 };
 
+// What reaches the bound, in any order (LDS).  More than 64 -- many equal classes -- overflow: the list takes over.
+struct Pool {
+  unsigned key[64];
+  int cls[64];
+  int count;
+  __device__ __forceinline__ void push(unsigned k, int c) {
+    const int at = atomicAdd(&count, 1);
+    if (at < 64) { key[at] = k; cls[at] = c; }
+  }
+};
+// A lane's (key, class) of `count` in lanes 0 .. count - 1: how many of the others come before it.  All are different, so the
+// places are, too, whatever order they were pushed in.
+__device__ __forceinline__ int place_of(unsigned k, int c, int count) {
+  int r = 0;
+  for (int i = 0; i < count; ++i) {
+    const unsigned ki = (unsigned)__builtin_amdgcn_readlane((int)k, i);
+    const int ci = __builtin_amdgcn_readlane(c, i);
+    r += ki > k || (ki == k && ci < c) ? 1 : 0;
+  }
+  return r;
+}
+
 __device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
 // ---------------------------------------------------------------- rows: the classes of a site are adjacent
-// NT threads (one wave, or a workgroup) per row, 16-byte loads with the row's unaligned ends taken one by one.  Bound by
-// HBM for many rows, by the latency of one pass for few: 1024 threads on one row keep 16 loads of 1 KiB in flight.
+// One wave or one workgroup of four per row, 16-byte loads with the row's unaligned ends taken one by one.  Bound by HBM
+// for many rows; where there are few, a row is cut over several workgroups (one workgroup reads a row of 131072 at the
+// latency of its own loads: 25 us) and a second kernel joins the parts.
 //
-// The alternatives cost no second pass: a lane's running maximum is the largest of its own classes, so the `top`-th
-// largest of the lanes' maxima is a lower bound for the top-th best class, and only lanes whose maximum reaches it can
-// hold one.  Those few lanes go over their own classes again (in cache) and offer what reaches the bound to a list.
+// The alternatives cost no second pass: a lane's running maximum is the largest of its own classes.  The lanes form
+// sixteen groups; the `top`-th largest of the groups' maxima (top <= 16) is a lower bound for the top-th best class, and only
+// lanes whose maximum reaches it can hold one (of random classes about 16 ln 2 reach the bound for top 8).  Those few lanes
+// go over their own classes again (in cache) and put what reaches the bound into a small pool, whose members are then
+// placed by counting (inserting them one by one into a sorted list, which remains for pools that overflow, was half the
+// time of a short row).
 template <int DT> struct Vec {
   typedef typename Elem<DT>::type T;
   static constexpr int N = 16 / sizeof(T);
@@ -190,53 +233,68 @@ __device__ __forceinline__ void add_many(Stat* st, const float* x) {
   }
 }
 
+// what a cut row's parts leave for the join: [site][part] statistics and lists
+struct Parts {
+  float* stat;        // 3 floats each
+  unsigned* key;      // `top` each
+  int* cls;
+};
+
 template <int DT, int NT>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void symbol_rows_kernel(Logits l, const int* symbols, int top, float* log_prob,
-                                                                          float* entropy, float* stats, float* top_lp, int* top_sym,
-                                                                          int sites) {
+__global__ __launch_bounds__(256) void symbol_rows_kernel(Logits l, const int* symbols, int top, float* log_prob, float* entropy,
+                                                          float* stats, float* top_lp, int* top_sym, int sites, int nparts,
+                                                          Parts parts) {
   typedef typename Elem<DT>::type T;
-  constexpr int N = Vec<DT>::N, WAVES = NT / 64, ROWS = NT < 256 ? 256 / NT : 1;
+  constexpr int N = Vec<DT>::N, WAVES = NT / 64, ROWS = 256 / NT;
+  static_assert(NT == 64 || NT == 256, "a wave or a workgroup per row (part)");
   __shared__ float part[WAVES > 1 ? WAVES * 3 : 1];
   __shared__ unsigned keys[WAVES > 1 ? WAVES * DVC_MAX_TOP : 1];
   __shared__ int classes_of[WAVES > 1 ? WAVES * DVC_MAX_TOP : 1];
+  __shared__ Pool pools[ROWS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  Pool* const pool = &pools[ROWS > 1 ? wave : 0];
   const int tid = ROWS > 1 ? lane : (int)threadIdx.x;
-  const int site = __builtin_amdgcn_readfirstlane((int)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0));
+  const int unit = __builtin_amdgcn_readfirstlane((int)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0));
+  const int site = NT == 64 ? unit : unit / nparts, piece = NT == 64 ? 0 : unit - site * nparts;
   if (site >= sites) return;            // (whole waves, and only where a row is a wave: no barrier below is missed)
   const int n = site / l.groups, g = site - n * l.groups;
   const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes;
-  const RowPart rp = row_part<DT>(row, l.classes);
-  const uint4* const body = reinterpret_cast<const uint4*>(row + rp.head);
+  RowPart rp = row_part<DT>(row, l.classes);
+  const int all_vecs = rp.body, b0 = (int)((long long)all_vecs * piece / nparts), b1 = (int)((long long)all_vecs * (piece + 1) / nparts);
+  const uint4* const body = reinterpret_cast<const uint4*>(row + rp.head) + b0;
+  const int body_v = rp.head + b0 * N;  // this part's first class
+  rp.body = b1 - b0;
+
+  if (tid == 0) pool->count = 0;
+  float given_x = 0.f;                  // (requested before the row is read: at the end it would be a wait of its own)
+  int sym = -1;
+  if (nparts == 1) {
+    sym = symbols[site];
+    if (sym >= 0 && sym < l.classes) given_x = Elem<DT>::up(row[sym]);
+  }
 
   Stat st;
   st.clear();
   // ends: at most N - 1 classes on either side
-  const int ends = rp.head + l.classes - rp.tail0;
+  const int ends = piece == 0 ? rp.head + l.classes - rp.tail0 : 0;
   const int end_v = tid < rp.head ? tid : rp.tail0 + tid - rp.head;
   const bool has_end = tid < ends;
   const float end_x = has_end ? Elem<DT>::up(row[end_v]) : NEG_INF;
   if (has_end) st.add(end_x);
-  constexpr int U = 4;
-  int j = tid;
-  for (; j + (U - 1) * NT < rp.body; j += U * NT) {
+  constexpr int U = 4;                  // vectors in flight per lane
+  for (int j = tid; j < rp.body; j += U * NT) {
     Vec<DT> q[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) q[u].q = body[j + u * NT];
+    for (int u = 0; u < U; ++u)
+      if (j + u * NT < rp.body) q[u].q = body[j + u * NT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[N];
+    for (int u = 0; u < U; ++u)
+      if (j + u * NT < rp.body) {
+        float x[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = Elem<DT>::up(q[u].e[i]);
-      add_many<N>(&st, x);
-    }
-  }
-  for (; j < rp.body; j += NT) {
-    Vec<DT> q;
-    q.q = body[j];
-    float x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = Elem<DT>::up(q.e[i]);
-    add_many<N>(&st, x);
+        for (int i = 0; i < N; ++i) x[i] = Elem<DT>::up(q[u].e[i]);
+        add_many<N>(&st, x);
+      }
   }
 
   // what the lane's best class is worth; a lane that met a NaN or +inf looks again (its maximum ignores NaN)
@@ -262,59 +320,39 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void symbol_rows_kernel(Logits
   if constexpr (WAVES > 1) {
     if (lane == 0) { part[wave * 3] = all.m; part[wave * 3 + 1] = all.s; part[wave * 3 + 2] = all.t; }
   }
-  // the wave's `top` best lanes, one after the other
+  // the groups' maxima: four lanes each where the row is a wave, sixteen where it is a workgroup
   unsigned bound = 0;
   if (top > 0) {
-    unsigned k = best, mine = 0;
-    for (int i = 0; i < top; ++i) {
-      bound = wave_max(k);
-      if (lane == i) mine = bound;
-      const unsigned long long eq = __ballot(k == bound);
-      if (lane == __ffsll((long long)eq) - 1) k = 0;
-    }
+    unsigned k = best, o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0xB1, 0xF, 0xF, true);
+    k = k > o ? k : o;
+    o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x4E, 0xF, 0xF, true);
+    k = k > o ? k : o;
     if constexpr (WAVES > 1) {
-      if (lane < top) keys[wave * DVC_MAX_TOP + lane] = mine;
+      o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x141, 0xF, 0xF, true);
+      k = k > o ? k : o;
+      o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x140, 0xF, 0xF, true);
+      k = k > o ? k : o;
+      if ((lane & 15) == 0) keys[wave * 4 + (lane >> 4)] = k;
+    } else {
+      bound = nth_of_16((unsigned)__shfl((int)k, 4 * (lane & 15), 64), top, lane);
     }
   }
   if constexpr (WAVES > 1) {
     __syncthreads();
     all.clear();
     for (int w = 0; w < WAVES; ++w) all.join(part[w * 3], part[w * 3 + 1], part[w * 3 + 2]);
-    if (top > 0) {
-      // the top-th best of all waves' (WAVES * 16 places, in every wave alike)
-      constexpr int PER = (WAVES * DVC_MAX_TOP + 63) / 64;
-      unsigned k[PER];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = i * 64 + lane;
-        k[i] = at < WAVES * DVC_MAX_TOP && at % DVC_MAX_TOP < top ? keys[at] : 0;
-      }
-      for (int r = 0; r < top; ++r) {
-        unsigned mx = k[0];
-#pragma unroll
-        for (int i = 1; i < PER; ++i) mx = k[i] > mx ? k[i] : mx;
-        bound = wave_max(mx);
-        const unsigned long long eq = __ballot(mx == bound);
-        if (lane == __ffsll((long long)eq) - 1) {
-          bool done = false;
-#pragma unroll
-          for (int i = 0; i < PER; ++i)
-            if (!done && k[i] == bound) { k[i] = 0; done = true; }
-        }
-      }
-    }
+    if (top > 0) bound = nth_of_16(keys[lane & 15], top, lane);
   }
   float log_s, h;
   finish(all, &log_s, &h);
 
   if (top > 0) {
-    WaveList list;
-    list.clear();
-    const bool in = best >= bound && best != 0;      // (fewer lanes than `top` with a class: bound 0, all look)
-    if (__ballot(in)) {
-      const unsigned ke = order_key(end_x);
-      list.offer(in && has_end && ke >= bound ? ke : 0, end_v, lane, top);
-      for (int v = tid; v - tid + (tid & ~63) < rp.body; v += NT) {      // uniform over the wave
+    const bool in = best >= bound && best != 0;      // (fewer groups than `top` with a class: bound 0, all look)
+    const unsigned end_k = in && has_end ? order_key(end_x) : 0;
+    // goes over the lane's own vectors whose best reaches the bound and `least`; uniform over the wave
+    auto look = [&](auto&& least, auto&& take) __attribute__((always_inline)) {
+      if (!__ballot(in)) return;
+      for (int v = tid; v - tid + (tid & ~63) < rp.body; v += NT) {
         Vec<DT> q;
         const bool have = in && v < rp.body;
         if (have) q.q = body[v];
@@ -328,37 +366,140 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void symbol_rows_kernel(Logits
           nan |= x[i] != x[i];
         }
         const unsigned km = nan ? 0xffffffffu : order_key(vm);
-        if (!__ballot(have && km >= bound && km >= list.last_key)) continue;
+        if (!__ballot(have && km >= bound && km >= least())) continue;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const unsigned k = order_key(x[i]);
-          list.offer(have && k >= bound ? k : 0, rp.head + v * N + i, lane, top);
+          take(have && k >= bound ? k : 0, body_v + v * N + i);
         }
       }
-    }
-    if constexpr (WAVES > 1) {
-      __syncthreads();                   // the keys of the bound have been read
-      if (lane < top) {
-        keys[wave * DVC_MAX_TOP + lane] = list.key;
-        classes_of[wave * DVC_MAX_TOP + lane] = list.cls;
+    };
+    if (end_k != 0 && end_k >= bound) pool->push(end_k, end_v);
+    look([] { return 0u; }, [&](unsigned k, int c) { if (k != 0) pool->push(k, c); });
+    if constexpr (WAVES > 1) __syncthreads();
+    else __threadfence_block();
+    const int count = __builtin_amdgcn_readfirstlane(pool->count);
+    unsigned key = 0;
+    int cls = 0, place = top;
+    if (count <= 64) {
+      if (ROWS > 1 || wave == 0) {
+        if (lane < count) { key = pool->key[lane]; cls = pool->cls[lane]; }
+        place = place_of(key, cls, count);
+        place = lane < count ? place : top;
       }
-      __syncthreads();
-      if (wave == 0)
-        for (int b = DVC_MAX_TOP; b < WAVES * DVC_MAX_TOP; b += 64) {      // place 0..15 is this wave's own list
-          const int at = b + lane;
-          const bool have = at < WAVES * DVC_MAX_TOP && at % DVC_MAX_TOP < top;
-          list.offer(have ? keys[at] : 0, have ? classes_of[at] : 0, lane, top);
+    } else {
+      WaveList list;
+      list.clear();
+      list.offer(end_k >= bound ? end_k : 0, end_v, lane, top);
+      look([&] { return list.last_key; }, [&](unsigned k, int c) { list.offer(k, c, lane, top); });
+      if constexpr (WAVES > 1) {
+        if (lane < top) {                 // (the groups' maxima in `keys` were read before the barrier above)
+          keys[wave * DVC_MAX_TOP + lane] = list.key;
+          classes_of[wave * DVC_MAX_TOP + lane] = list.cls;
         }
+        __syncthreads();
+        if (wave == 0) {                  // place 0..15 is this wave's own list
+          const bool have = lane >= DVC_MAX_TOP && lane % DVC_MAX_TOP < top;
+          static_assert(WAVES * DVC_MAX_TOP == 64, "the waves' lists are a lane each");
+          list.offer(have ? keys[lane] : 0, have ? classes_of[lane] : 0, lane, top);
+        }
+      }
+      key = list.key;
+      cls = list.cls;
+      place = (ROWS > 1 || wave == 0) && lane < top ? lane : top;
     }
-    if ((ROWS > 1 || wave == 0) && lane < top) {
-      top_lp[(long long)site * top + lane] = log_p(key_value(list.key), all.m, log_s);
-      top_sym[(long long)site * top + lane] = list.cls;
+    if (place < top) {
+      const long long at = (long long)unit * top + place;       // (a whole row's unit is its site)
+      if (nparts > 1) {
+        parts.key[at] = key;
+        parts.cls[at] = cls;
+      } else {
+        top_lp[at] = log_p(key_value(key), all.m, log_s);
+        top_sym[at] = cls;
+      }
     }
   }
-  if ((ROWS > 1 || wave == 0) && lane == 0) {
-    log_prob[site] = given<DT>(row, 1, l.classes, symbols[site], all.m, log_s);
+  if (nparts > 1) {
+    if (threadIdx.x == 0) {
+      parts.stat[(long long)unit * 3] = all.m;
+      parts.stat[(long long)unit * 3 + 1] = all.s;
+      parts.stat[(long long)unit * 3 + 2] = all.t;
+    }
+  } else if (tid == 0) {
+    log_prob[site] = given_log_p(sym, l.classes, given_x, all.m, log_s);
     entropy[site] = h;
     stats[site] = all.m;
+    stats[(long long)sites + site] = log_s;
+  }
+}
+
+// The parts of a cut row (at most 64: a lane each) joined, a wave per row.
+constexpr int kMaxParts = 64;
+
+template <int DT>
+__global__ __launch_bounds__(64) void symbol_rows_join_kernel(Logits l, const int* symbols, int top, float* log_prob, float* entropy,
+                                                              float* stats, float* top_lp, int* top_sym, int sites, int nparts,
+                                                              Parts parts) {
+  typedef typename Elem<DT>::type T;
+  __shared__ Pool pool;
+  const int lane = threadIdx.x, site = blockIdx.x;
+  const bool have = lane < nparts;
+  const long long at = (long long)site * nparts + (have ? lane : 0);
+  const int n = site / l.groups, g = site - n * l.groups;
+  const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes;
+  const int sym = symbols[site];
+  Stat st;
+  st.clear();
+  if (have) { st.m = parts.stat[at * 3]; st.s = parts.stat[at * 3 + 1]; st.t = parts.stat[at * 3 + 2]; }
+  unsigned key[DVC_MAX_TOP];        // (all requested before the first is used)
+  int cls[DVC_MAX_TOP];
+#pragma unroll
+  for (int j = 0; j < DVC_MAX_TOP; ++j) {
+    key[j] = have && j < top ? parts.key[at * top + j] : 0;
+    cls[j] = have && j < top ? parts.cls[at * top + j] : 0;
+  }
+  const float given_x = sym >= 0 && sym < l.classes ? Elem<DT>::up(row[sym]) : 0.f;
+  if (lane == 0) pool.count = 0;
+  wave_join(&st);
+  float log_s, h;
+  finish(st, &log_s, &h);
+  if (top > 0) {
+    // four parts' first places a group: the same bound as over a row's lanes
+    unsigned k = key[0], o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0xB1, 0xF, 0xF, true);
+    k = k > o ? k : o;
+    o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x4E, 0xF, 0xF, true);
+    k = k > o ? k : o;
+    const unsigned bound = nth_of_16((unsigned)__shfl((int)k, 4 * (lane & 15), 64), top, lane);
+    __threadfence_block();
+#pragma unroll
+    for (int j = 0; j < DVC_MAX_TOP; ++j)
+      if (key[j] != 0 && key[j] >= bound) pool.push(key[j], cls[j]);
+    __threadfence_block();
+    const int count = __builtin_amdgcn_readfirstlane(pool.count);
+    unsigned my_key = 0;
+    int my_cls = 0, place = top;
+    if (count <= 64) {
+      if (lane < count) { my_key = pool.key[lane]; my_cls = pool.cls[lane]; }
+      place = place_of(my_key, my_cls, count);
+      place = lane < count ? place : top;
+    } else {
+      WaveList list;
+      list.clear();
+#pragma unroll
+      for (int j = 0; j < DVC_MAX_TOP; ++j) list.offer(key[j], cls[j], lane, top);
+      my_key = list.key;
+      my_cls = list.cls;
+      place = lane;
+    }
+    if (place < top) {
+      top_lp[(long long)site * top + place] = log_p(key_value(my_key), st.m, log_s);
+      top_sym[(long long)site * top + place] = my_cls;
+    }
+  }
+  if (lane == 0) {
+    log_prob[site] = given_log_p(sym, l.classes, given_x, st.m, log_s);
+    entropy[site] = h;
+    stats[site] = st.m;
     stats[(long long)sites + site] = log_s;
   }
 }
@@ -586,21 +727,42 @@ inline bool is_rows(const DvcLogits* l, int h, int w) {
   return h == 1 && w == 1 && (l->class_stride == 1 || (l->classes == 1 && l->groups == 1));
 }
 
+// Into how many parts a row is cut: while the rows alone give fewer than 512 workgroups (two per CU), as long as a part
+// keeps two 16-byte vectors per thread (one row of 131072 bf16: 25 us whole, 9 us in 32 parts and a join).
+inline int row_parts(const DvcLogits* l, int batch, int h, int w) {
+  const long long sites = (long long)batch * l->groups;
+  if (!is_rows(l, h, w) || l->classes <= 1024 || sites >= 512) return 1;
+  const long long vecs = (long long)l->classes * (l->dtype == DVC_F32 ? 4 : 2) / 16, want = (512 + sites - 1) / sites;
+  const long long most = vecs / 512 < kMaxParts ? vecs / 512 : kMaxParts;
+  return (int)(want < most ? want : most < 1 ? 1 : most);
+}
+
 template <int DT>
 int launch_forward(const DvcLogits* l, const int32_t* symbols, int top, float* log_prob, float* entropy, float* stats, float* top_lp,
-                   int32_t* top_sym, int batch, int h, int w, hipStream_t st) {
+                   int32_t* top_sym, float* scratch, int batch, int h, int w, hipStream_t st) {
   const unsigned hw = (unsigned)((long long)h * w);
   const long long sites = (long long)batch * l->groups * hw;
   if (is_rows(l, h, w)) {
-#define ROWS(NT, GRID, BLOCK) hipLaunchKernelGGL((symbol_rows_kernel<DT, NT>), dim3(GRID), dim3(BLOCK), 0, st, mk(l), symbols, top, log_prob, \
-                                                 entropy, stats, top_lp, top_sym, (int)sites)
-    // A wave per row while a row is at most a few vectors per lane; otherwise a workgroup: of 16 waves where the rows
-    // alone do not fill the 256 CUs (fewer than 1024 of them) and a row gives every lane a vector
-    if (l->classes <= 1024) ROWS(64, (unsigned)((sites + 3) / 4), 256);
-    else if (sites >= 1024 || l->classes < 8192) ROWS(256, (unsigned)sites, 256);
-    else ROWS(1024, (unsigned)sites, 1024);
-#undef ROWS
-    return dvc::check_launch("symbol_rows_kernel");
+    // a wave per row while a row is at most a few vectors per lane
+    if (l->classes <= 1024) {
+      hipLaunchKernelGGL((symbol_rows_kernel<DT, 64>), dim3((unsigned)((sites + 3) / 4)), dim3(256), 0, st, mk(l), symbols, top, log_prob,
+                         entropy, stats, top_lp, top_sym, (int)sites, 1, Parts{});
+      return dvc::check_launch("symbol_rows_kernel");
+    }
+    const int nparts = row_parts(l, batch, h, w);
+    const long long units = sites * nparts;
+    Parts parts{};
+    if (nparts > 1) {
+      DVC_REQUIRE(scratch != nullptr, "dvc_symbol_log_probs: null scratch");
+      parts = Parts{scratch, reinterpret_cast<unsigned*>(scratch + units * 3), reinterpret_cast<int*>(scratch + units * (3 + top))};
+    }
+    hipLaunchKernelGGL((symbol_rows_kernel<DT, 256>), dim3((unsigned)units), dim3(256), 0, st, mk(l), symbols, top, log_prob, entropy,
+                       stats, top_lp, top_sym, (int)sites, nparts, parts);
+    if (int rc = dvc::check_launch("symbol_rows_kernel")) return rc;
+    if (nparts == 1) return DVC_OK;
+    hipLaunchKernelGGL(symbol_rows_join_kernel<DT>, dim3((unsigned)sites), dim3(64), 0, st, mk(l), symbols, top, log_prob, entropy, stats,
+                       top_lp, top_sym, (int)sites, nparts, parts);
+    return dvc::check_launch("symbol_rows_join_kernel");
   }
   const long long waves = (sites + 63) / 64;
   DVC_REQUIRE(waves < (1LL << 31), "dvc_symbol_log_probs: too many sites");
@@ -650,7 +812,9 @@ int launch_backward(const DvcLogits* l, const int32_t* symbols, const float* sta
 
 extern "C" int64_t dvc_symbol_log_probs_scratch_floats(const DvcLogits* logits, int32_t top, int32_t batch, int32_t h, int32_t w) {
   if (int rc = check_logits(logits, batch, h, w, "dvc_symbol_log_probs_scratch_floats")) return rc;
-  return 0;
+  DVC_REQUIRE(top >= 0 && top <= DVC_MAX_TOP, "dvc_symbol_log_probs_scratch_floats: top=%d (0..%d)", top, DVC_MAX_TOP);
+  const int nparts = row_parts(logits, batch, h, w);
+  return nparts == 1 ? 0 : (int64_t)batch * logits->groups * nparts * (3 + 2 * top);
 }
 
 extern "C" int dvc_symbol_log_probs(const DvcLogits* logits, const int32_t* symbols, int32_t top, float* log_prob, float* entropy,
@@ -662,7 +826,7 @@ extern "C" int dvc_symbol_log_probs(const DvcLogits* logits, const int32_t* symb
               top, DVC_MAX_TOP, logits->classes);
   DVC_REQUIRE(top == 0 || (top_log_prob != nullptr && top_symbol != nullptr), "dvc_symbol_log_probs: null pointer");
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define GO(DT) launch_forward<DT>(logits, symbols, top, log_prob, entropy, stats, top_log_prob, top_symbol, batch, h, w, st)
+#define GO(DT) launch_forward<DT>(logits, symbols, top, log_prob, entropy, stats, top_log_prob, top_symbol, scratch, batch, h, w, st)
   return logits->dtype == DVC_F32 ? GO(DVC_F32) : logits->dtype == DVC_BF16 ? GO(DVC_BF16) : GO(DVC_F16);
 #undef GO
 }

@@ -19,7 +19,9 @@ Srcs = Union[Tensor, Sequence[Tensor]]
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device (torch.cuda.current_stream().cuda_stream without the stream object: a
+    tenth of a launch's host time instead of half of it)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _check4(t: Tensor, name: str, dtype=torch.float32):
@@ -627,7 +629,7 @@ def _blocks(h: int, w: int) -> int:
 
 
 def _on_current_device(t: Tensor, name: str):
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
