@@ -8,12 +8,12 @@ int launch_aligned(int ks, int stride, const Args& a, const Plan& p, hipStream_t
 
 namespace {
 
-// gW[co][ci][tap] = sum over splits of partial[split][tap][co][ci], gB[co] likewise (indices past the weight's).  A block
-// takes 64 results; each of its WAVES waves adds every WAVES-th split, with the loads of four splits in flight, and the sums
-// are added in a fixed order.  16 waves for many splits (256 of a 64 x 64 3x3 layer: 9 us, 20 with four waves and one load
-// after the other), 4 for few.
+// gW[co][ci][tap] = sum over slabs of partial[slab][tap][co][ci], gB[co] likewise over splits (indices past the weight's).  A block
+// takes 64 results; each of its WAVES waves adds every WAVES-th slab, with the loads of four slabs in flight, and the sums are
+// added in a fixed order.  16 waves for many slabs (256 of a 64 x 64 3x3 layer: 9 us, 20 with four waves and one load after
+// the other), 4 for few.
 template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int nsplit, int taps, int cout, int cin,
+__global__ __launch_bounds__(64 * WAVES) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int slabs, int nsplit, int taps, int cout, int cin,
                                                                  int cout_pad, int cin_pad, const float* bias_partial, float* gb) {
   __shared__ float part[WAVES][64];
   const long long total = (long long)cout * taps * cin;
@@ -23,6 +23,7 @@ __global__ __launch_bounds__(64 * WAVES) void wgrad_ckpt_reduce_kernel(const flo
     const long long i = i0 + lane;
     const float* p = nullptr;
     long long step = 0, dst = -1;
+    int count = slabs;
     if (i < total) {
       const unsigned r = (unsigned)i, ci = r % (unsigned)cin, q = r / (unsigned)cin;      // (a weight has below 2^31 elements)
       const unsigned tap = q % (unsigned)taps, co = q / (unsigned)taps;
@@ -32,15 +33,16 @@ __global__ __launch_bounds__(64 * WAVES) void wgrad_ckpt_reduce_kernel(const flo
     } else if (i < total_all) {
       p = bias_partial + (i - total);
       step = cout_pad;
+      count = nsplit;
     }
     float s = 0.f;
     if (p != nullptr) {
       int k = kg;
-      for (; k + 3 * WAVES < nsplit; k += 4 * WAVES) {
+      for (; k + 3 * WAVES < count; k += 4 * WAVES) {
         const float v0 = p[k * step], v1 = p[(k + WAVES) * step], v2 = p[(k + 2 * WAVES) * step], v3 = p[(k + 3 * WAVES) * step];
         s += (v0 + v1) + (v2 + v3);
       }
-      for (; k < nsplit; k += WAVES) s += p[k * step];
+      for (; k < count; k += WAVES) s += p[k * step];
     }
     part[kg][lane] = s;
     __syncthreads();
@@ -65,12 +67,10 @@ int make_plan(int cout, int cin, int ks, int stride, int batch, int h, int w, Pl
   const int pad = ks / 2;
   p->ho = (h + 2 * pad - ks) / stride + 1;
   p->wo = (w + 2 * pad - ks) / stride + 1;
-  // layers that fill a 32 x 32 block badly and whose fp32 form is narrower: 7x7 with a handful of channels
-  p->restore = ks == 7 && (cout <= 4 || cin <= 8);
   p->tw = ks == 3 && stride == 1 && p->wo <= 16 ? 16 : 32;
   p->mt = (cout > 32 && ks != 7) ? 2 : 1;
   p->ct = (cin > 32 && ks != 7) ? 2 : 1;
-  p->th = ks == 1 ? 4 : (stride == 2 && p->mt * p->ct > 1 ? 2 : 4) * (32 / p->tw);
+  p->th = (ks == 3 && stride == 2 ? 2 : 4) * (32 / p->tw);
   p->tiles_x = (p->wo + p->tw - 1) / p->tw;
   p->tiles_y = (p->ho + p->th - 1) / p->th;
   const long long nt = (long long)batch * p->tiles_x * p->tiles_y;
@@ -85,6 +85,14 @@ int make_plan(int cout, int cin, int ks, int stride, int batch, int h, int w, Pl
   // one 8-wave workgroup fits a CU: about one round of them
   int s = (256 + p->blocks - 1) / p->blocks;
   p->nsplit = s > p->n_tiles ? p->n_tiles : s;
+  // A running sum is rounded twice per matrix instruction, so a slab ends after 256 row pieces of a wave (768 instructions;
+  // 64->64 3x3 at 32x256x256, 512 pieces per wave: relative error 7e-7 in two slabs, 1.0e-6 in one); 7x7, whose slabs are
+  // five times as large, after 512
+  const int kg = ks == 7 ? 1 : 4 / (p->mt * p->ct), pieces = p->th * p->tw / 16 / kg;
+  p->seg_tiles = (ks == 7 ? 512 : 256) / pieces;
+  const int most = (p->n_tiles + p->nsplit - 1) / p->nsplit;      // tiles of a workgroup
+  p->segments = (most + p->seg_tiles - 1) / p->seg_tiles;
+  p->slabs = p->segments * p->nsplit * kg;
   return DVC_OK;
 }
 
@@ -110,11 +118,7 @@ extern "C" int64_t dvc_conv2d_wgrad_ckpt_scratch_floats(int32_t cout, int32_t ci
                                                         int32_t batch, int32_t in_h, int32_t in_w) {
   Plan p;
   if (int rc = make_plan(cout, cin, ksize, stride, batch, in_h, in_w, &p, "dvc_conv2d_wgrad_ckpt_scratch_floats")) return rc;
-  if (p.restore) {
-    const int64_t n = dvc_conv2d_wgrad_scratch_floats(cout, cin, ksize, stride, batch, in_h, in_w);
-    return n < 0 ? n : n + (int64_t)batch * cin * in_h * in_w;
-  }
-  return (int64_t)p.nsplit * p.taps * p.cout_pad * p.cin_pad + (int64_t)p.nsplit * p.cout_pad;
+  return (int64_t)p.slabs * p.taps * p.cout_pad * p.cin_pad + (int64_t)p.nsplit * p.cout_pad;
 }
 
 extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t batch, int32_t in_h, int32_t in_w,
@@ -126,18 +130,6 @@ extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t
   DVC_REQUIRE(grad_out != nullptr && scratch != nullptr && grad_weight != nullptr, "%s: null pointer", who);
   Plan p;
   if (int rc = make_plan(out_channels, cin, ksize, stride, batch, in_h, in_w, &p, who)) return rc;
-  if (p.restore) {
-    const int64_t plane = (int64_t)in_h * in_w;
-    const DvcSrc x{scratch, cin * plane, plane, cin, 0};
-    int c0 = 0;
-    for (int s = 0; s < n_src; ++s) {
-      const DvcDst d{scratch + c0 * plane, cin * plane, plane};
-      if (int rc = dvc_act_restore(&srcs[s], &d, batch, in_h, in_w, stream)) return rc;
-      c0 += srcs[s].channels;
-    }
-    return dvc_conv2d_wgrad(&x, 1, batch, in_h, in_w, 0, 1.f, grad_out, out_channels, ksize, stride, scratch + batch * cin * plane,
-                            grad_weight, grad_bias, stream);
-  }
   Args a{};
   int first = 0;
   for (int s = 0; s < DVC_MAX_SRC; ++s) {
@@ -158,22 +150,24 @@ extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t
   a.wo = p.wo;
   a.g = grad_out;
   a.partial = scratch;
-  a.bias_partial = grad_bias != nullptr ? scratch + (long long)p.nsplit * p.taps * p.cout_pad * p.cin_pad : nullptr;
+  a.bias_partial = grad_bias != nullptr ? scratch + (long long)p.slabs * p.taps * p.cout_pad * p.cin_pad : nullptr;
   a.cout_pad = p.cout_pad;
   a.cin_pad = p.cin_pad;
   a.n_cib = p.n_cib;
   a.tiles_x = p.tiles_x;
   a.tiles_y = p.tiles_y;
   a.n_tiles = p.n_tiles;
+  a.seg_tiles = p.seg_tiles;
+  a.segments = p.segments;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool aligned = in_w % 4 == 0 && p.wo % 4 == 0 && reinterpret_cast<uintptr_t>(grad_out) % 16 == 0 &&
                        4LL * out_channels * p.ho * p.wo < (1LL << 31);
   if (int rc = aligned ? launch_aligned(ksize, stride, a, p, st) : launch_any(ksize, stride, a, p, st)) return rc;
   const long long total = (long long)out_channels * cin * p.taps + out_channels;
   const dim3 grid((unsigned)((total + 63) / 64 < 16384 ? (total + 63) / 64 : 16384));
-#define REDUCE(WAVES) hipLaunchKernelGGL(wgrad_ckpt_reduce_kernel<WAVES>, grid, dim3(64 * WAVES), 0, st, scratch, grad_weight, p.nsplit, \
+#define REDUCE(WAVES) hipLaunchKernelGGL(wgrad_ckpt_reduce_kernel<WAVES>, grid, dim3(64 * WAVES), 0, st, scratch, grad_weight, p.slabs, p.nsplit, \
                                          p.taps, out_channels, cin, p.cout_pad, p.cin_pad, a.bias_partial, grad_bias)
-  if (p.nsplit >= 64) REDUCE(16);
+  if (p.slabs >= 64) REDUCE(16);
   else REDUCE(4);
 #undef REDUCE
   return dvc::check_launch("wgrad_ckpt_reduce_kernel");

@@ -11,15 +11,19 @@
 // v_mfma_f32_32x32x16_bf16: rows = 32 output channels, columns = 32 input channels at one tap, k = 16 adjacent
 // pixels of a row (a half-wave holds 8 of them: one 16-byte LDS read).  The taps of a row read the same 16-byte windows,
 // shifted by whole elements in registers (v_alignbit): nine products of a 3x3 layer need three window reads.
-// A workgroup (8 waves) owns (32 MT) x (32 CT) of the result for all taps; the 8 / (MT CT) waves of one 32 x 32 corner
-// take the row pieces of a tile in turn and are added through LDS in a fixed order at the end.  The pixel axis is cut
-// into slabs whose partial results a second kernel adds in a fixed order (deterministic, no atomics).
+// A workgroup (8 waves) owns (32 MT) x (32 CT) of the result for all taps.  Four waves (one per SIMD) multiply: a wave keeps a
+// 32 x 32 corner for every tap in registers; the 4 / (MT CT) waves of one corner take the row pieces of a tile in turn.  The
+// other four stage (7x7: wave ky < 7 multiplies tap row ky of a 32 x 32 block, and all eight stage).  With every wave doing
+// both, staging and multiplying took turns: 457 us for 64->64 3x3 at 32x256x256, of 233 us staging alone and 275 us
+// multiplying alone.  The pixel axis is cut into slabs -- over workgroups, over the waves of a corner and, so that
+// no running sum gets too long for fp32, in time -- whose partial results a second kernel adds in a fixed order
+// (deterministic, no atomics).
 //
-// Staging per tile of TH x TW output pixels, two LDS buffers and one barrier per tile: while a tile is multiplied the next
-// one's codes, scales and gradients (loaded during the tile before) are decoded to bf16 / stored as fp32 into the other
-// buffer, and the loads of the one after are issued.  A lane decodes four codes of a row (one dword).  The gradient stays
-// fp32 in LDS (4 instead of 6 bytes) and is split when it is read; the bias gradient is summed by the lanes that stage it.
-// Channel strides in LDS are odd multiples of 16 bytes: 16 lanes of a read (16 channels) fall on all 64 banks.
+// Staging per tile of TH x TW output pixels, two LDS buffers and one barrier per tile: the codes, scales and gradients of the
+// next tile (loaded a tile ago) are decoded to bf16 / stored as fp32 while a tile is multiplied, and the loads of the one
+// after are issued.  A lane decodes four codes of a row (one dword).  The gradient stays fp32 in LDS (4 instead of 6
+// bytes) and is split when it is read, in the shadow of the matrix instructions; the bias gradient is summed by the lanes that
+// stage it.  Channel strides in LDS are odd multiples of 16 bytes: 16 lanes of a read (16 channels) fall on all 64 banks.
 #pragma once
 #include <atomic>
 #include <type_traits>
@@ -41,10 +45,11 @@ struct Args {
   int cin, h, w, blocks;        // blocks of 32 per plane
   int cout, ho, wo;
   const float* g;               // [N][cout][ho][wo], contiguous
-  float* partial;               // [S][taps][cout_pad][cin_pad]
-  float* bias_partial;          // [S][cout_pad], or null
+  float* partial;               // [slabs][taps][cout_pad][cin_pad], slab = (segment * splits + split) * KG + wave of the corner
+  float* bias_partial;          // [splits][cout_pad], or null
   int cout_pad, cin_pad, n_cib;
   int tiles_x, tiles_y, n_tiles;
+  int seg_tiles, segments;      // tiles of a workgroup per slab, slabs of a workgroup and wave (segments * seg_tiles tiles or fewer)
 };
 
 __device__ __forceinline__ unsigned long long uniform64(unsigned long long v) {
@@ -146,13 +151,15 @@ __device__ __forceinline__ bf16x8 window(const unsigned (&d)[D]) {
 // Geometry.  KS x KS taps, stride S, tiles of TH x TW output pixels; a staged input row is XD dwords of codes from column
 // gx0 = ox0 * S - LEFT on (a multiple of 4), kept in LDS as XROW bf16: as it is (stride 1), or its even columns, then
 // (3x3) its odd ones, so that the eight pixels of a half-wave are adjacent at stride 2 as well.
-template <int KS, int S, int MT, int CT, int TW_>
+template <int KS_, int S_, int MT, int CT, int TW_>
 struct Geo {
-  static constexpr int KG = KS == 7 ? 1 : 8 / (MT * CT);         // waves sharing one corner (7x7: one tap row per wave)
+  static constexpr int KS = KS_, S = S_;
+  static constexpr int NM = KS == 7 ? 7 : 4, NS = KS == 7 ? 8 : 4;      // multiplying and staging waves
+  static constexpr int KG = KS == 7 ? 1 : NM / (MT * CT);        // waves sharing one corner (7x7: one tap row per wave)
   static constexpr int XCH = 32 * CT, GCH = 32 * MT;
   static constexpr int TAPS = KS * KS, ACC = KS == 7 ? 7 : TAPS; // accumulator tiles per wave
   static_assert(KS != 7 || (S == 1 && MT == 1 && CT == 1), "7x7: 32 x 32 blocks, stride 1");
-  static constexpr int TW = TW_, TH = KS == 1 ? 4 : (S == 2 && KG < 8 ? 2 : 4) * (32 / TW_), PAD = KS / 2;
+  static constexpr int TW = TW_, TH = (KS == 3 && S == 2 ? 2 : 4) * (32 / TW_), PAD = KS / 2;
   static constexpr int LEFT = KS == 1 ? 0 : 4;
   static constexpr int YS = KS == 1 ? S : 1;                     // input rows between staged rows
   static constexpr int IH = KS == 1 ? TH : (TH - 1) * S + KS;
@@ -163,65 +170,60 @@ struct Geo {
   static constexpr int XUNITS = (IH * XROW / 8) | 1;             // 16-byte units per channel, odd
   static constexpr int GUNITS = (TH * TW / 4) | 1;
   static constexpr int XE = IH * XD, XSLOTS = (XE + 63) / 64;
-  static constexpr int XPW = XCH / 8;                            // channels of x staged per wave
-  static constexpr int GE = TH * TW / 4, GLOADS = GCH * GE / 512;
-  static_assert(GCH * GE % 512 == 0, "gradient units deal out evenly");
+  static constexpr int XPW = XCH / NS;                           // channels of x per staging wave
+  static constexpr int GE = TH * TW / 4, GLOADS = GCH * GE / (64 * NS);      // 16-byte units of g per channel, per staging lane
+  static_assert(GCH * GE % (64 * NS) == 0 && 64 % GE == 0, "gradient units deal out evenly, a channel's on adjacent lanes");
   static constexpr int XBYTES = XCH * XUNITS * 16, BUF = XBYTES + GCH * GUNITS * 16;
-  static constexpr int RED = (KG - 1) * MT * CT * 4096;
-  static constexpr int LDS_BYTES = 2 * BUF > RED ? 2 * BUF : RED;
+  static constexpr int LDS_BYTES = 2 * BUF;
   static_assert(LDS_BYTES <= 160 * 1024, "LDS");
   static constexpr int STEPS = TH * TW / 16;                     // row pieces of 16 pixels per tile
   static_assert(STEPS % KG == 0, "row pieces deal out evenly");
 };
 
+// The staging side of a kernel: NS waves deal out the channels of x and the 16-byte units of g of a tile.
 // AL: rows of codes start on dwords and rows of gradients on 16 bytes (w % 4 == 0, wo % 4 == 0).
-template <int KS, int S, int MT, int CT, int TW, bool AL>
-__global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
-  using G = Geo<KS, S, MT, CT, TW>;
-  constexpr int KG = G::KG, XPW = G::XPW, XSLOTS = G::XSLOTS, GLOADS = G::GLOADS, TAPS = G::TAPS, ACC = G::ACC;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-
-  const int tid = threadIdx.x;
-  const int lane = tid & 63, half = lane >> 5, l32 = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int corner = KS == 7 ? 0 : wave % (MT * CT), grp = KS == 7 ? 0 : wave / (MT * CT);
-  const int mt = corner / CT, ct = corner % CT;
-  const int cob = blockIdx.y / a.n_cib, cib = blockIdx.y - cob * a.n_cib;
-  const int co0 = cob * G::GCH, ci0 = cib * G::XCH;
-  const int nsplit = gridDim.x;
-  const int per_n = a.tiles_x * a.tiles_y;
-  const unsigned plane_bytes = 32u * (unsigned)a.blocks;
-  const unsigned gplane = (unsigned)(a.ho * a.wo);
-
-  // Every second slab is computed with its inputs' signs changed and changed back when it is stored: the matrix
-  // instruction cuts what lies far below its running sum downwards, and over the slabs that drift cancels (64->64 3x3 at
-  // 32x256x256: relative error 2.0e-6 without, of which 93 % is drift).  It costs nothing: the sign rides on the scale.
-  const unsigned flip = (blockIdx.x & 1u) << 31;
-
+template <class G, bool AL>
+struct Stager {
+  static constexpr int KS = G::KS, S = G::S, TW = G::TW, XPW = G::XPW, XSLOTS = G::XSLOTS, GLOADS = G::GLOADS;
+  const Args& a;
+  const int lane, sw, stid;
+  const unsigned flip;
+  int per_n, xlive;             // tiles per sample, this wave's channels that exist
+  bool together;                // this wave's channels are adjacent planes
+  unsigned plane_bytes, gplane, gsample;
   Plane xp[XPW];
-#pragma unroll
-  for (int c = 0; c < XPW; ++c) xp[c] = plane_of(a, ci0 + XPW * wave + c);
-  const int xlive = a.cin - (ci0 + XPW * wave);      // this wave's channels that exist
-  // gradient units: unit u = tid + 512 i is unit u % GE of channel u / GE
+  // gradient units: unit u = stid + 64 NS i is unit u % GE of channel u / GE
   unsigned gsrc[GLOADS];        // this lane's channel; past the last: none
   int gdst[GLOADS];
-  const unsigned gsample = 4u * (unsigned)a.cout * gplane;      // AL: below 2^31 (checked on the host)
-#pragma unroll
-  for (int i = 0; i < GLOADS; ++i) {
-    const int u = tid + 512 * i, ch = u / G::GE, e = u - ch * G::GE;
-    gsrc[i] = co0 + ch < a.cout ? (unsigned)(co0 + ch) : 0xffffffffu;
-    gdst[i] = G::XBYTES + (ch * G::GUNITS + e) * 16;
-  }
   float gsum[GLOADS];
-#pragma unroll
-  for (int i = 0; i < GLOADS; ++i) gsum[i] = 0.f;
-
   unsigned xk[XPW][XSLOTS], xs[XPW][XSLOTS], xs2[AL ? 1 : XPW][AL ? 1 : XSLOTS];
   int mask[XSLOTS];             // codes of a dword inside the row (not AL)
   int cut[XSLOTS];              // codes of a dword before a block's end (not AL)
   float4 gr[GLOADS];
 
-  auto load = [&](int t) __attribute__((always_inline)) {      // request tile t (past the last: zeros)
+  __device__ __forceinline__ Stager(const Args& args, int lane_, int sw_, int co0, int ci0, unsigned flip_)
+      : a(args), lane(lane_), sw(sw_), stid(64 * sw_ + lane_), flip(flip_) {
+    per_n = a.tiles_x * a.tiles_y;
+    plane_bytes = 32u * (unsigned)a.blocks;
+    gplane = (unsigned)(a.ho * a.wo);
+    gsample = 4u * (unsigned)a.cout * gplane;      // AL: below 2^31 (checked on the host)
+    xlive = a.cin - (ci0 + XPW * sw);
+#pragma unroll
+    for (int c = 0; c < XPW; ++c) xp[c] = plane_of(a, ci0 + XPW * sw + c);
+    together = xlive >= XPW && xp[XPW - 1].codes == xp[0].codes + (unsigned long long)(XPW - 1) * plane_bytes &&
+               xp[XPW - 1].scales == xp[0].scales + (unsigned long long)(XPW - 1) * (unsigned)a.blocks &&
+               xp[XPW - 1].step == xp[0].step && (unsigned long long)XPW * plane_bytes < (1ull << 31);
+#pragma unroll
+    for (int i = 0; i < GLOADS; ++i) {
+      const int u = stid + 64 * G::NS * i, ch = u / G::GE, e = u - ch * G::GE;
+      gsrc[i] = co0 + ch < a.cout ? (unsigned)(co0 + ch) : 0xffffffffu;
+      gdst[i] = G::XBYTES + (ch * G::GUNITS + e) * 16;
+      gsum[i] = 0.f;
+    }
+  }
+
+  // request tile t (past the last: zeros)
+  __device__ __forceinline__ void load(int t) {
     const bool there = t < a.n_tiles;
     const int tt = there ? t : 0;
     const int n = tt / per_n, r = tt - n * per_n;
@@ -240,6 +242,20 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
         cut[j] = 32 - (int)(off[j] & 31u);
       }
     }
+    // A wave whose channels all lie in one source needs one descriptor per tile and a scalar offset per channel; otherwise
+    // every channel's address is put together (as many scalar instructions as a slot has vector ones).
+    if (AL && together) {
+      const unsigned long long b = (unsigned long long)(unsigned)n * xp[0].step;
+      const __amdgpu_buffer_rsrc_t rc = rsrc(xp[0].codes + 32ull * b, there ? (unsigned)XPW * plane_bytes : 0u);
+      const __amdgpu_buffer_rsrc_t rs = rsrc(xp[0].scales + b, there ? (unsigned)(XPW * a.blocks) : 0u);
+#pragma unroll
+      for (int c = 0; c < XPW; ++c)
+#pragma unroll
+        for (int j = 0; j < XSLOTS; ++j) {
+          xk[c][j] = __builtin_amdgcn_raw_buffer_load_b32(rc, off[j], c * plane_bytes, 0);
+          xs[c][j] = __builtin_amdgcn_raw_buffer_load_b8(rs, off[j] >> 5, c * a.blocks, 0);
+        }
+    } else
 #pragma unroll
     for (int c = 0; c < XPW; ++c) {
       const unsigned long long b = (unsigned long long)(unsigned)n * xp[c].step;
@@ -266,7 +282,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     // gradients: four adjacent pixels of a row
 #pragma unroll
     for (int i = 0; i < GLOADS; ++i) {
-      const int e = (tid + 512 * i) % G::GE;
+      const int e = stid % G::GE;
       const int oy = oy0 + 4 * e / TW, ox = ox0 + 4 * e % TW;
       const bool ok = gsrc[i] != 0xffffffffu && oy < a.ho && ox < a.wo;
       if constexpr (AL) {
@@ -284,9 +300,11 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
         }
       }
     }
-  };
+  }
 
-  auto store_as = [&](char* buf, auto e4m3) __attribute__((always_inline)) {      // decode what load() requested into an LDS buffer
+  // decode what load() requested into an LDS buffer
+  template <bool E4M3>
+  __device__ __forceinline__ void store_as(char* buf) {
 #pragma unroll
     for (int j = 0; j < XSLOTS; ++j) {
       const int e = lane + 64 * j, iy = e / G::XD, q = e - iy * G::XD;
@@ -295,16 +313,16 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
         const float s0 = scale_of(xs[c][j], flip);
         uint2 v;
         if constexpr (AL) {
-          v = decode<decltype(e4m3)::value>(xk[c][j], s0, s0, s0, s0);
+          v = decode<E4M3>(xk[c][j], s0, s0, s0, s0);
         } else {
           const float s4 = scale_of(xs2[c][j], flip);
-          v = decode<decltype(e4m3)::value>(xk[c][j], s0, cut[j] > 1 ? s0 : s4, cut[j] > 2 ? s0 : s4, cut[j] > 3 ? s0 : s4);
+          v = decode<E4M3>(xk[c][j], s0, cut[j] > 1 ? s0 : s4, cut[j] > 2 ? s0 : s4, cut[j] > 3 ? s0 : s4);
           // codes past the row's end are padding: zeros (also where the scale is that of a poisoned block)
           v.x = mask[j] > 1 ? v.x : mask[j] > 0 ? v.x & 0xffffu : 0u;
           v.y = mask[j] > 3 ? v.y : mask[j] > 2 ? v.y & 0xffffu : 0u;
         }
         if (64 * (j + 1) <= G::XE || e < G::XE) {
-          char* const row = buf + ((XPW * wave + c) * G::XUNITS * 8 + iy * G::XROW) * 2;
+          char* const row = buf + ((XPW * sw + c) * G::XUNITS * 8 + iy * G::XROW) * 2;
           if constexpr (S == 1) {
             *reinterpret_cast<uint2*>(row + 8 * q) = v;
           } else {
@@ -325,13 +343,68 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
       *reinterpret_cast<float4*>(buf + gdst[i]) = gr[i];
       gsum[i] += (gr[i].x + gr[i].y) + (gr[i].z + gr[i].w);
     }
-  };
+  }
 
-  auto store = [&](char* buf) __attribute__((always_inline)) {
-    if (a.e4m3) store_as(buf, std::true_type{});
-    else store_as(buf, std::false_type{});
-  };
+  __device__ __forceinline__ void store(char* buf) {
+    if (a.e4m3) store_as<true>(buf);
+    else store_as<false>(buf);
+  }
 
+  // the bias gradient of what was staged: a channel's units are GE adjacent lanes
+  __device__ __forceinline__ void bias(float* out) {
+#pragma unroll
+    for (int i = 0; i < GLOADS; ++i) {
+      float v = gsum[i];
+#pragma unroll
+      for (int m = G::GE / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+      if (stid % G::GE == 0) out[(stid + 64 * G::NS * i) / G::GE] = v;
+    }
+  }
+};
+
+template <int KS, int S, int MT, int CT, int TW, bool AL>
+__global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
+  using G = Geo<KS, S, MT, CT, TW>;
+  constexpr int KG = G::KG, TAPS = G::TAPS, ACC = G::ACC;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cob = blockIdx.y / a.n_cib, cib = blockIdx.y - cob * a.n_cib;
+  const int co0 = cob * G::GCH, ci0 = cib * G::XCH;
+  const int nsplit = gridDim.x;
+  // Workgroups go to the eight XCDs in turn, each with an L2 of its own, and neighbouring tiles share the cache lines of the
+  // codes (a staged row is 40 bytes): tiles that follow each other go to one XCD.
+  const int part = nsplit % 8 == 0 ? ((int)blockIdx.x & 7) * (nsplit >> 3) + ((int)blockIdx.x >> 3) : (int)blockIdx.x;
+
+  // Every second slab is computed with its inputs' signs changed and changed back when it is stored: the matrix
+  // instruction cuts what lies far below its running sum downwards, and over the slabs that drift cancels (64->64 3x3 at
+  // 32x256x256: relative error 2.0e-6 without, of which 93 % is drift).  It costs nothing: the sign rides on the scale.
+  const unsigned flip = ((unsigned)part & 1u) << 31;
+
+  if (KS != 7 && wave >= G::NM) {
+    // ------------------------------------------------------------ staging
+    Stager<G, AL> st(a, lane, wave - G::NM, co0, ci0, flip);
+    int buf = 0;
+    st.load(part);
+    st.store(lds);
+    st.load(part + nsplit);
+    __syncthreads();
+    for (int t = part; t < a.n_tiles; t += nsplit) {
+      st.store(lds + (G::BUF - buf));        // tile t + nsplit (zeros past the last)
+      st.load(t + 2 * nsplit);
+      __syncthreads();
+      buf = G::BUF - buf;
+    }
+    if (a.bias_partial != nullptr && cib == 0) st.bias(a.bias_partial + (long long)part * a.cout_pad + co0);
+    return;
+  }
+
+  // -------------------------------------------------------------- multiplying
+  const int half = lane >> 5, l32 = lane & 31;
+  const int corner = KS == 7 ? 0 : wave % (MT * CT), grp = KS == 7 ? 0 : wave / (MT * CT);
+  const int mt = corner / CT, ct = corner % CT;
   f32x16 acc[ACC];
 #pragma unroll
   for (int t = 0; t < ACC; ++t)
@@ -340,134 +413,116 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
 
   const int ga = G::XBYTES + (mt * 32 + l32) * G::GUNITS * 16 + half * 32;
   const int xa = (ct * 32 + l32) * G::XUNITS * 16 + half * 16;
+  constexpr int ROWS = KS == 7 ? 1 : KS;            // staged rows a row piece meets in this wave
+  constexpr int STEPS = G::STEPS / KG;              // row pieces per tile in this wave
 
-  auto multiply = [&](const char* buf, int step) __attribute__((always_inline)) {       // one row piece
-    const int row = step / (TW / 16), px = step % (TW / 16) * 16;
-    const float4* const gp = reinterpret_cast<const float4*>(buf + ga + (row * TW + px) * 4);
-    const Split s = split(gp[0], gp[1]);
-    constexpr int ROWS = KS == 7 ? 1 : KS;
+  // one tile: the operands of a row piece are read and split while the piece before is multiplied
+  auto multiply = [&](const char* buf) __attribute__((always_inline)) {
+    auto gradient = [&](int i) __attribute__((always_inline)) {
+      const int step = i * KG + grp, row = step / (TW / 16), px = step % (TW / 16) * 16;
+      const float4* const gp = reinterpret_cast<const float4*>(buf + ga + (row * TW + px) * 4);
+      return split(gp[0], gp[1]);
+    };
+    Split s = gradient(0);
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int ky = KS == 7 ? wave : i;
-      const char* const xr = buf + xa + ((KS == 1 ? row : row * S + ky) * G::XROW + px) * 2;
-      bf16x8 b[KS];
-      if constexpr (KS == 1) {
-        b[0] = *reinterpret_cast<const bf16x8*>(xr);
-      } else if constexpr (S == 1) {
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(xr), hi = *reinterpret_cast<const u32x4*>(xr + 16);
-        const unsigned d[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        if constexpr (KS == 3) {      // staged column 4 is pixel 0
-          b[0] = window<3>(d); b[1] = window<4>(d); b[2] = window<5>(d);
-        } else {
+    for (int i = 0; i < STEPS; ++i) {
+      const int step = i * KG + grp, row = step / (TW / 16), px = step % (TW / 16) * 16;
+      Split next = s;
+      if (i + 1 < STEPS) next = gradient(i + 1);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const int ky = KS == 7 ? wave : r;
+        const char* const xr = buf + xa + ((KS == 1 ? row : row * S + ky) * G::XROW + px) * 2;
+        bf16x8 b[KS];
+        if constexpr (KS == 1) {
+          b[0] = *reinterpret_cast<const bf16x8*>(xr);
+        } else if constexpr (KS == 3 && S == 1) {
+          // staged column 4 is pixel 0: the middle tap is elements 4..11, its neighbours one element either way
+          const unsigned lo = *reinterpret_cast<const unsigned*>(xr + 4), hi = *reinterpret_cast<const unsigned*>(xr + 24);
+          const uint2 m0 = *reinterpret_cast<const uint2*>(xr + 8), m1 = *reinterpret_cast<const uint2*>(xr + 16);
+          const unsigned d[6] = {lo, m0.x, m0.y, m1.x, m1.y, hi};
+          b[0] = window<1>(d); b[1] = window<2>(d); b[2] = window<3>(d);
+        } else if constexpr (S == 1) {
+          const u32x4 lo = *reinterpret_cast<const u32x4*>(xr), hi = *reinterpret_cast<const u32x4*>(xr + 16);
+          const unsigned d[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
           b[0] = window<1>(d); b[1] = window<2>(d); b[2] = window<3>(d); b[3] = window<4>(d);
           b[4] = window<5>(d); b[5] = window<6>(d); b[6] = window<7>(d);
+        } else {
+          const u32x4 lo = *reinterpret_cast<const u32x4*>(xr + 2 * TW);
+          const unsigned d[5] = {lo[0], lo[1], lo[2], lo[3], *reinterpret_cast<const unsigned*>(xr + 2 * TW + 16)};
+          b[0] = window<1>(d); b[2] = window<2>(d);
+          b[1] = *reinterpret_cast<const bf16x8*>(xr);
         }
-      } else {
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(xr + 2 * TW);
-        const unsigned d[5] = {lo[0], lo[1], lo[2], lo[3], *reinterpret_cast<const unsigned*>(xr + 2 * TW + 16)};
-        b[0] = window<1>(d); b[2] = window<2>(d);
-        b[1] = *reinterpret_cast<const bf16x8*>(xr);
+#pragma unroll
+        for (int kx = 0; kx < KS; ++kx) acc[r * KS + kx] = mfma(s.a3, b[kx], acc[r * KS + kx]);
+#pragma unroll
+        for (int kx = 0; kx < KS; ++kx) acc[r * KS + kx] = mfma(s.a2, b[kx], acc[r * KS + kx]);
+#pragma unroll
+        for (int kx = 0; kx < KS; ++kx) acc[r * KS + kx] = mfma(s.a1, b[kx], acc[r * KS + kx]);
       }
-#pragma unroll
-      for (int kx = 0; kx < KS; ++kx) acc[i * KS + kx] = mfma(s.a3, b[kx], acc[i * KS + kx]);
-#pragma unroll
-      for (int kx = 0; kx < KS; ++kx) acc[i * KS + kx] = mfma(s.a2, b[kx], acc[i * KS + kx]);
-#pragma unroll
-      for (int kx = 0; kx < KS; ++kx) acc[i * KS + kx] = mfma(s.a1, b[kx], acc[i * KS + kx]);
+      s = next;
     }
   };
 
-  // Of the two waves of a SIMD one stages before it multiplies and one after: between the same two barriers the decoding
-  // of the one runs beside the matrix instructions of the other.
+  // slab after slab (a workgroup that runs out of tiles early still writes its slabs); register r of an accumulator is row
+  // (r & 3) + 8 (r >> 2) + 4 half, column l32
+  const long long slab_floats = (long long)TAPS * a.cout_pad * a.cin_pad;
+  float* out = a.partial + ((long long)part * KG + grp) * slab_floats + (long long)(co0 + mt * 32 + 4 * half) * a.cin_pad +
+               ci0 + ct * 32 + l32;
+  // 7x7: the multiplying waves stage as well (one wave cannot hold a tile's loads); of the two waves of a SIMD one does so
+  // before it multiplies and one after, so that the decoding of the one runs beside the matrix instructions of the other
+  auto st = [&]() __attribute__((always_inline)) {
+    if constexpr (KS == 7) return Stager<G, AL>(a, lane, wave, co0, ci0, flip);
+    else return 0;
+  }();
   const bool late = wave >= 4;
-  int t = blockIdx.x, buf = 0;
-  load(t);
-  store(lds);
-  load(t + nsplit);
-  __syncthreads();
-  for (; t < a.n_tiles; t += nsplit) {
-    if (!late) {
-      store(lds + (G::BUF - buf));        // tile t + nsplit (zeros past the last)
-      load(t + 2 * nsplit);
-    }
-    if (KS != 7 || wave < 7) {
-#pragma unroll
-      for (int i = 0; i < G::STEPS / KG; ++i) multiply(lds + buf, i * KG + grp);
-    }
-    if (late) {
-      store(lds + (G::BUF - buf));
-      load(t + 2 * nsplit);
-    }
-    __syncthreads();
-    buf = G::BUF - buf;
-  }
-
-  // bias gradient: the lanes of a channel are GE adjacent ones (a multiple of 32): butterfly within 32, then one atomic-free
-  // add per half through LDS below
-  float* const bs = reinterpret_cast<float*>(lds);      // [GCH][GE / 32]
-  if (a.bias_partial != nullptr && cib == 0) {
-    constexpr int SEG = G::GE < 64 ? G::GE : 64;         // adjacent lanes of one channel
-    static_assert(SEG == 16 || SEG == 32 || SEG == 64, "butterfly");
-#pragma unroll
-    for (int i = 0; i < GLOADS; ++i) {
-      float v = gsum[i];
-#pragma unroll
-      for (int m = SEG / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-      if ((lane & (SEG - 1)) == 0) bs[(tid + 512 * i) / SEG] = v;
-    }
-    __syncthreads();
-    constexpr int PARTS = G::GE / SEG;
-    if (tid < G::GCH) {
-      float v = 0.f;
-#pragma unroll
-      for (int k = 0; k < PARTS; ++k) v += bs[tid * PARTS + k];
-      a.bias_partial[(long long)blockIdx.x * a.cout_pad + co0 + tid] = v;
-    }
-    __syncthreads();
-  }
-
-  // add the waves of a corner, tap by tap; register r of a tile is row (r & 3) + 8 (r >> 2) + 4 half, column l32
-  float* const red = reinterpret_cast<float*>(lds);
-  auto unflip = [&](float v) { return __uint_as_float(__float_as_uint(v) ^ flip); };
-  float* const pbase = a.partial + (long long)blockIdx.x * TAPS * a.cout_pad * a.cin_pad;
+  int t = part, buf = 0;
   if constexpr (KS == 7) {
-    if (wave < 7) {
-#pragma unroll
-      for (int kx = 0; kx < 7; ++kx) {
-        float* const pt = pbase + (long long)(wave * 7 + kx) * a.cout_pad * a.cin_pad + ci0 + l32;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) pt[(long long)(co0 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = unflip(acc[kx][r]);
-      }
-    }
-    return;
+    st.load(t);
+    st.store(lds);
+    st.load(t + nsplit);
   }
-#pragma unroll
-  for (int tp = 0; tp < ACC; ++tp) {
-    if (KG > 1 && grp > 0) {
-      float* const dst = red + ((grp - 1) * (MT * CT) + corner) * 1024 + lane;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dst[64 * r] = acc[tp][r];
-    }
-    if (KG > 1) __syncthreads();
-    if (grp == 0) {
-      f32x16 v = acc[tp];
-#pragma unroll
-      for (int k = 1; k < KG; ++k) {
-        const float* const src = red + ((k - 1) * (MT * CT) + corner) * 1024 + lane;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] += src[64 * r];
+  __syncthreads();
+#pragma unroll 1
+  for (int seg = 0; seg < a.segments; ++seg) {
+#pragma unroll 1
+    for (int k = 0; k < a.seg_tiles && t < a.n_tiles; ++k, t += nsplit) {
+      if constexpr (KS == 7) {
+        if (!late) {
+          st.store(lds + (G::BUF - buf));
+          st.load(t + 2 * nsplit);
+        }
       }
-      float* const pt = pbase + (long long)tp * a.cout_pad * a.cin_pad + ci0 + ct * 32 + l32;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) pt[(long long)(co0 + mt * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * a.cin_pad] = unflip(v[r]);
+      if (KS != 7 || wave < 7) multiply(lds + buf);
+      if constexpr (KS == 7) {
+        if (late) {
+          st.store(lds + (G::BUF - buf));
+          st.load(t + 2 * nsplit);
+        }
+      }
+      __syncthreads();
+      buf = G::BUF - buf;
     }
-    if (KG > 1) __syncthreads();
+    if (KS == 7 && wave == 7) continue;
+#pragma unroll
+    for (int tp = 0; tp < ACC; ++tp) {
+      float* const pt = out + (long long)(KS == 7 ? wave * 7 + tp : tp) * a.cout_pad * a.cin_pad;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        pt[((r & 3) + 8 * (r >> 2)) * a.cin_pad] = __uint_as_float(__float_as_uint(acc[tp][r]) ^ flip);
+        acc[tp][r] = 0.f;
+      }
+    }
+    out += (long long)nsplit * KG * slab_floats;
+  }
+  if constexpr (KS == 7) {
+    if (a.bias_partial != nullptr && cib == 0) st.bias(a.bias_partial + (long long)part * a.cout_pad + co0);
   }
 }
 
 struct Plan {
   int ho, wo, tw, th, tiles_x, tiles_y, n_tiles, cout_pad, cin_pad, n_cib, blocks, nsplit, taps, mt, ct;
-  bool restore;      // no kernel for this shape here: restore and run the fp32 one
+  int seg_tiles, segments, slabs;      // tiles of a workgroup per slab, slabs in time, slabs in all
 };
 
 template <class K>
