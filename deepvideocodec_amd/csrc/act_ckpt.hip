@@ -20,6 +20,8 @@ inline Dst mk(const DvcDst* d) { return Dst{d->ptr, d->batch_stride, d->chan_str
 
 constexpr int UPB = 4;              // units per lane
 constexpr int WG_UNITS = 256 * UPB;
+// unit j of a thread inside its workgroup's: a wave's 4 x 64 units are adjacent, and so are the 32 scales of their blocks
+__device__ __forceinline__ unsigned unit_of(int j) { return (threadIdx.x & ~63u) * UPB + 64 * j + (threadIdx.x & 63); }
 
 // Where the units of this launch lie: `upp` units per plane (8 per block), `planes` planes.
 struct Walk {
@@ -144,11 +146,12 @@ __global__ __launch_bounds__(256) void act_checkpoint_kernel(Src x, Walk k, unsi
   Unit t[UPB];
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    const unsigned local = j * 256 + threadIdx.x;
+    const unsigned local = unit_of(j);
     t[j] = locate(k, base, local);
     v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (base + local < k.units) v[j] = load_unit<VEC>(plane_of(x, t[j]), t[j].u, hw);
   }
+  unsigned sj = 0;
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
     float4 a = v[j];
@@ -162,12 +165,14 @@ __global__ __launch_bounds__(256) void act_checkpoint_kernel(Src x, Walk k, unsi
     const unsigned amax = max8(m01 > m23 ? m01 : m23);   // blocks never straddle the launch's end: units % 8 == 0
     unsigned s;
     const unsigned code = encode4<FMT>(a, amax, &s);
-    const long long unit = base + j * 256 + threadIdx.x;
-    if (unit < k.units) {
-      codes[unit] = code;
-      if ((threadIdx.x & 7) == 0) scales[unit >> 3] = (uint8_t)s;
-    }
+    const long long unit = base + unit_of(j);
+    if (unit < k.units) codes[unit] = code;
+    sj = (threadIdx.x & 7) == (unsigned)j ? s : sj;
   }
+  // the wave's 32 scales in one store: lane 8 b + j that of the block b of its j-th 64 units
+  const int j = threadIdx.x & 7;
+  const long long unit = base + unit_of(j) - j;      // (first unit of that block)
+  if (j < UPB && unit < k.units) scales[unit >> 3] = (uint8_t)sj;
 }
 
 template <int FMT, bool VEC>
@@ -177,7 +182,7 @@ __global__ __launch_bounds__(256) void act_restore_kernel(const unsigned* codes,
   unsigned code[UPB], s[UPB];
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    const long long unit = base + j * 256 + threadIdx.x;
+    const long long unit = base + unit_of(j);
     code[j] = s[j] = 0;
     if (unit < k.units) {
       code[j] = codes[unit];
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(256) void act_restore_kernel(const unsigned* codes,
   }
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    const unsigned local = j * 256 + threadIdx.x;
+    const unsigned local = unit_of(j);
     if (base + local < k.units) {
       const Unit t = locate(k, base, local);
       store_unit<VEC>(plane_of(out, t), t.u, hw, decode4<FMT>(code[j], s[j]));
@@ -200,7 +205,7 @@ __global__ __launch_bounds__(256) void act_signs_kernel(Src x, Walk k, unsigned 
   float4 v[UPB];
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    const unsigned local = j * 256 + threadIdx.x;
+    const unsigned local = unit_of(j);
     v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (base + local < k.units) {
       const Unit t = locate(k, base, local);
@@ -211,7 +216,7 @@ __global__ __launch_bounds__(256) void act_signs_kernel(Src x, Walk k, unsigned 
   for (int j = 0; j < UPB; ++j) {
     const unsigned nib = (v[j].x > 0.f ? 1u : 0u) | (v[j].y > 0.f ? 2u : 0u) | (v[j].z > 0.f ? 4u : 0u) | (v[j].w > 0.f ? 8u : 0u);
     const unsigned word = or8(nib << (4 * (threadIdx.x & 7)));
-    const long long unit = base + j * 256 + threadIdx.x;
+    const long long unit = base + unit_of(j);
     if (unit < k.units && (threadIdx.x & 7) == 0) signs[unit >> 3] = word;
   }
 }
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(256) void act_grad_signs_kernel(Src g, const unsign
   Unit t[UPB];
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    const unsigned local = j * 256 + threadIdx.x;
+    const unsigned local = unit_of(j);
     t[j] = locate(k, base, local);
     v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     bits[j] = 0;
@@ -237,7 +242,7 @@ __global__ __launch_bounds__(256) void act_grad_signs_kernel(Src g, const unsign
   }
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    if (base + j * 256 + threadIdx.x < k.units) {
+    if (base + unit_of(j) < k.units) {
       float4 r = v[j];
       r.x = (bits[j] & 1u) ? r.x : r.x * slope; r.y = (bits[j] & 2u) ? r.y : r.y * slope;
       r.z = (bits[j] & 4u) ? r.z : r.z * slope; r.w = (bits[j] & 8u) ? r.w : r.w * slope;
@@ -272,7 +277,7 @@ __global__ __launch_bounds__(256) void mul_act_grad_ckpt_kernel(Src g, const uns
   Unit t[UPB];
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    const unsigned local = j * 256 + threadIdx.x;
+    const unsigned local = unit_of(j);
     t[j] = locate(k, base, local);
     v[j] = e[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     code[j] = 0;
@@ -284,7 +289,7 @@ __global__ __launch_bounds__(256) void mul_act_grad_ckpt_kernel(Src g, const uns
   }
 #pragma unroll
   for (int j = 0; j < UPB; ++j) {
-    if (base + j * 256 + threadIdx.x < k.units) {
+    if (base + unit_of(j) < k.units) {
       float4 r = v[j];
       r.x = (code[j] & 0x80u) ? r.x * slope : r.x; r.y = (code[j] & 0x8000u) ? r.y * slope : r.y;
       r.z = (code[j] & 0x800000u) ? r.z * slope : r.z; r.w = (code[j] & 0x80000000u) ? r.w * slope : r.w;
