@@ -189,7 +189,7 @@ struct Stager {
   const int lane, sw, stid;
   const unsigned flip;
   int per_n, xlive;             // tiles per sample, this wave's channels that exist
-  bool together;                // this wave's channels are adjacent planes
+  bool together;                // this wave's channels all exist and lie in one source: adjacent planes
   unsigned plane_bytes, gplane, gsample;
   Plane xp[XPW];
   // gradient units: unit u = stid + 64 NS i is unit u % GE of channel u / GE
@@ -197,8 +197,9 @@ struct Stager {
   int gdst[GLOADS];
   float gsum[GLOADS];
   unsigned xk[XPW][XSLOTS], xs[XPW][XSLOTS], xs2[AL ? 1 : XPW][AL ? 1 : XSLOTS];
-  int mask[XSLOTS];             // codes of a dword inside the row (not AL)
+  int mask[XSLOTS];             // codes of a dword inside the row (not AL; none: it lies outside the plane)
   int cut[XSLOTS];              // codes of a dword before a block's end (not AL)
+  unsigned shift[XSLOTS];       // bits by which a dword was read early (not AL)
   float4 gr[GLOADS];
 
   __device__ __forceinline__ Stager(const Args& args, int lane_, int sw_, int co0, int ci0, unsigned flip_)
@@ -208,11 +209,19 @@ struct Stager {
     gplane = (unsigned)(a.ho * a.wo);
     gsample = 4u * (unsigned)a.cout * gplane;      // AL: below 2^31 (checked on the host)
     xlive = a.cin - (ci0 + XPW * sw);
+    // (finding a channel's plane is some 80 scalar instructions: 16 times that was a fifth of a one-tile workgroup's time)
+    const int c0 = ci0 + XPW * sw, c1 = c0 + XPW;
+    together = c1 <= a.cin && (unsigned long long)XPW * plane_bytes < (1ull << 31);
 #pragma unroll
-    for (int c = 0; c < XPW; ++c) xp[c] = plane_of(a, ci0 + XPW * sw + c);
-    together = xlive >= XPW && xp[XPW - 1].codes == xp[0].codes + (unsigned long long)(XPW - 1) * plane_bytes &&
-               xp[XPW - 1].scales == xp[0].scales + (unsigned long long)(XPW - 1) * (unsigned)a.blocks &&
-               xp[XPW - 1].step == xp[0].step && (unsigned long long)XPW * plane_bytes < (1ull << 31);
+    for (int k = 1; k < DVC_MAX_SRC; ++k) together = together && !(c0 < a.first[k] && a.first[k] < c1);
+    xp[0] = plane_of(a, c0);
+    if (!together) {
+#pragma unroll
+      for (int c = 1; c < XPW; ++c) xp[c] = plane_of(a, c0 + c);
+    } else {
+#pragma unroll
+      for (int c = 1; c < XPW; ++c) xp[c] = xp[0];
+    }
 #pragma unroll
     for (int i = 0; i < GLOADS; ++i) {
       const int u = stid + 64 * G::NS * i, ch = u / G::GE, e = u - ch * G::GE;
@@ -230,7 +239,7 @@ struct Stager {
     const int ty = r / a.tiles_x, tx = r - ty * a.tiles_x;
     const int oy0 = ty * G::TH, ox0 = tx * TW;
     const int gy0 = KS == 1 ? oy0 * S : oy0 * S - G::PAD, gx0 = ox0 * S - G::LEFT;
-    unsigned off[XSLOTS];
+    unsigned off[XSLOTS], from[XSLOTS], second[XSLOTS];
 #pragma unroll
     for (int j = 0; j < XSLOTS; ++j) {
       const int e = lane + 64 * j, iy = e / G::XD, q = e - iy * G::XD;
@@ -238,8 +247,14 @@ struct Stager {
       const bool ok = e < G::XE && gy >= 0 && gy < a.h && gx >= 0 && gx < a.w;
       off[j] = ok ? (unsigned)(gy * a.w + gx) : 0x80000000u;
       if constexpr (!AL) {
-        mask[j] = ok ? (a.w - gx < 4 ? a.w - gx : 4) : 0;
+        // a dword may start on any byte, span two blocks and reach past the plane's last byte: then the last four bytes are
+        // read and shifted.  Lanes without a place read the plane's first bytes, which the mask clears.
+        mask[j] = ok && there ? (a.w - gx < 4 ? a.w - gx : 4) : 0;
+        off[j] = ok ? off[j] : 0u;
         cut[j] = 32 - (int)(off[j] & 31u);
+        from[j] = off[j] < plane_bytes - 4u ? off[j] : plane_bytes - 4u;
+        shift[j] = 8u * (off[j] - from[j]);
+        second[j] = (off[j] + 3u) >> 5 < (unsigned)a.blocks - 1u ? (off[j] + 3u) >> 5 : (unsigned)a.blocks - 1u;
       }
     }
     // A wave whose channels all lie in one source needs one descriptor per tile and a scalar offset per channel; otherwise
@@ -253,7 +268,7 @@ struct Stager {
 #pragma unroll
         for (int j = 0; j < XSLOTS; ++j) {
           xk[c][j] = __builtin_amdgcn_raw_buffer_load_b32(rc, off[j], c * plane_bytes, 0);
-          xs[c][j] = __builtin_amdgcn_raw_buffer_load_b8(rs, off[j] >> 5, c * a.blocks, 0);
+          xs[c][j] = __builtin_amdgcn_raw_buffer_load_b8(rs, (int)off[j] >> 5, c * a.blocks, 0);      // (no place: still past the end)
         }
     } else
 #pragma unroll
@@ -264,18 +279,14 @@ struct Stager {
       for (int j = 0; j < XSLOTS; ++j) {
         if constexpr (AL) {
           xk[c][j] = __builtin_amdgcn_raw_buffer_load_b32(rsrc(xp[c].codes + 32ull * b, plane_bytes & live), off[j], 0, 0);
-          xs[c][j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(xp[c].scales + b, (unsigned)a.blocks & live), off[j] >> 5, 0, 0);
+          xs[c][j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(xp[c].scales + b, (unsigned)a.blocks & live), (int)off[j] >> 5, 0, 0);
         } else {
-          // the dword may reach past the plane's last byte: read the last four and shift
-          const bool ok = mask[j] > 0 && live;
-          const unsigned at = ok ? off[j] : 0u;
-          const unsigned from = at < plane_bytes - 4u ? at : plane_bytes - 4u;
-          const unsigned k = reinterpret_cast<const Dword*>(xp[c].codes + 32ull * b + from)->v >> (8u * (at - from));
-          xk[c][j] = ok ? k : 0u;
-          const uint8_t* const sp = reinterpret_cast<const uint8_t*>(xp[c].scales + b);
-          const unsigned last = (unsigned)a.blocks - 1u, b2 = (at + 3u) >> 5;
-          xs[c][j] = sp[at >> 5];
-          xs2[c][j] = sp[b2 < last ? b2 : last];
+          // (channels past the last: some plane; their sums are never looked at)
+          const unsigned long long cp = together ? xp[0].codes + 32ull * b + (unsigned long long)c * plane_bytes : xp[c].codes + 32ull * b;
+          const unsigned long long sp = together ? xp[0].scales + b + (unsigned long long)(c * a.blocks) : xp[c].scales + b;
+          xk[c][j] = reinterpret_cast<const Dword*>(cp + from[j])->v;
+          xs[c][j] = reinterpret_cast<const uint8_t*>(sp)[off[j] >> 5];
+          xs2[c][j] = reinterpret_cast<const uint8_t*>(sp)[second[j]];
         }
       }
     }
@@ -290,6 +301,7 @@ struct Stager {
         gr[i] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(
             rsrc((unsigned long long)a.g + (unsigned long long)(unsigned)n * gsample, there ? gsample : 0u), at, 0, 0));
       } else {
+        // (one unaligned 16-byte load per unit, masked when it is stored, was slower: 64->64 3x3 at 32x255x253 638 against 545 us)
         const float* const p = a.g + ((unsigned long long)(unsigned)n * a.cout + (ok ? gsrc[i] : 0u)) * gplane + (ok ? oy * a.wo + ox : 0);
         gr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (ok && there) {
@@ -316,7 +328,7 @@ struct Stager {
           v = decode<E4M3>(xk[c][j], s0, s0, s0, s0);
         } else {
           const float s4 = scale_of(xs2[c][j], flip);
-          v = decode<E4M3>(xk[c][j], s0, cut[j] > 1 ? s0 : s4, cut[j] > 2 ? s0 : s4, cut[j] > 3 ? s0 : s4);
+          v = decode<E4M3>(xk[c][j] >> shift[j], s0, cut[j] > 1 ? s0 : s4, cut[j] > 2 ? s0 : s4, cut[j] > 3 ? s0 : s4);
           // codes past the row's end are padding: zeros (also where the scale is that of a poisoned block)
           v.x = mask[j] > 1 ? v.x : mask[j] > 0 ? v.x & 0xffffu : 0u;
           v.y = mask[j] > 3 ? v.y : mask[j] > 2 ? v.y & 0xffffu : 0u;
@@ -423,12 +435,14 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
       const float4* const gp = reinterpret_cast<const float4*>(buf + ga + (row * TW + px) * 4);
       return split(gp[0], gp[1]);
     };
+    // (7x7: two waves of a SIMD multiply, and the operands of two row pieces would not leave registers for the staging)
+    constexpr bool AHEAD = KS != 7;
     Split s = gradient(0);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int step = i * KG + grp, row = step / (TW / 16), px = step % (TW / 16) * 16;
       Split next = s;
-      if (i + 1 < STEPS) next = gradient(i + 1);
+      if (AHEAD && i + 1 < STEPS) next = gradient(i + 1);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         const int ky = KS == 7 ? wave : r;
@@ -460,6 +474,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
 #pragma unroll
         for (int kx = 0; kx < KS; ++kx) acc[r * KS + kx] = mfma(s.a1, b[kx], acc[r * KS + kx]);
       }
+      if (!AHEAD && i + 1 < STEPS) next = gradient(i + 1);
       s = next;
     }
   };

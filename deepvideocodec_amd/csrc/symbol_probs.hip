@@ -716,7 +716,7 @@ int check_logits(const DvcLogits* l, int batch, int h, int w, const char* who) {
   DVC_REQUIRE(l->dtype == DVC_F32 || l->dtype == DVC_BF16 || l->dtype == DVC_F16, "%s: type %d unknown", who, l->dtype);
   DVC_REQUIRE(batch >= 1 && h >= 1 && w >= 1, "%s: bad dims", who);
   DVC_REQUIRE((long long)h * w < (1LL << 28), "%s: plane too large", who);
-  DVC_REQUIRE((long long)batch * l->groups < (1LL << 31), "%s: too many groups", who);
+  DVC_REQUIRE((long long)batch * l->groups < (1LL << 31) - 64, "%s: too many groups", who);
   DVC_REQUIRE(l->class_stride >= (int64_t)h * w, "%s: class stride < H*W", who);
   return DVC_OK;
 }

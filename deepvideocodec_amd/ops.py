@@ -652,6 +652,15 @@ def _ckpt(ck: ActCheckpoint, name: str, device=None) -> DvcCkpt:
     return DvcCkpt(ck.codes.data_ptr(), ck.scales.data_ptr(), c, fmt)
 
 
+def _distinct(t: Tensor, name: str):
+    """A destination whose samples or channels share memory (expanded views) would be written by several at once."""
+    n, c, h, w = t.shape
+    hw, s0, s1 = h * w, t.stride(0), t.stride(1) if t.size(1) > 1 else 0
+    samples = n == 1 or s0 >= (c - 1) * s1 + hw or (s0 >= hw and s0 * (n - 1) + hw <= s1)
+    if not samples or c > 1 and s1 < hw:
+        raise ValueError(f"{name}: overlapping planes (strides {t.stride()})")
+
+
 def _slope(slope: float, name: str) -> float:
     """LeakyReLU slopes outside [0, 1] do not keep the sign a derivative is read off (nor max(x, slope x))."""
     if not 0.0 <= float(slope) <= 1.0:
@@ -684,6 +693,7 @@ def act_restore(ck: ActCheckpoint, out: Optional[Tensor] = None) -> Tensor:
     elif tuple(out.shape) != tuple(ck.shape):
         raise ValueError(f"act_restore: out shape {tuple(out.shape)} != {tuple(ck.shape)}")
     dst = _dst(out)
+    _distinct(out, "act_restore out")
     if out.device != ck.codes.device:
         raise ValueError(f"act_restore: out on {out.device}, the checkpoint is on {ck.codes.device}")
     check(_lib.load().dvc_act_restore(C.byref(c), C.byref(dst), n, h, w, _stream()), "dvc_act_restore")
@@ -726,6 +736,8 @@ def mul_act_grad_ckpt(grad: Tensor, ck: ActCheckpoint, slope: float, out: Option
     for t, name in ((out, "out"), (plus, "plus")):
         if t is not None and (tuple(t.shape) != (n, c, h, w) or t.device != grad.device):
             raise ValueError(f"mul_act_grad_ckpt: {name} {tuple(t.shape)} on {t.device} does not match grad {(n, c, h, w)}")
+    _check4(out, "mul_act_grad_ckpt out")
+    _distinct(out, "mul_act_grad_ckpt out")
     check(_lib.load().dvc_mul_act_grad_ckpt(C.byref(_src(grad, "grad")), C.byref(_ckpt(ck, "mul_act_grad_ckpt", grad.device)),
                                             float(slope), C.byref(_src(plus, "plus")) if plus is not None else None,
                                             C.byref(_dst(out)), n, h, w, _stream()), "dvc_mul_act_grad_ckpt")

@@ -96,6 +96,12 @@ def test_symbol_refusals():
     refused(lib.dvc_symbol_log_probs_backward(lg(), P, None, P, P, P, P, 1, 8, 8, None), "null")
     refused(lib.dvc_symbol_log_probs_backward(lg(), P, P, P, P, P, None, 1, 8, 8, None), "null")
     assert lib.dvc_symbol_log_probs_scratch_floats(lg(classes=0), 0, 1, 8, 8) == -1
+    # one long row is cut over workgroups, which leave their parts in the scratch buffer
+    long_row = lg(cs=1, classes=131072)
+    assert lib.dvc_symbol_log_probs_scratch_floats(long_row, 8, 1, 1, 1) > 0
+    assert lib.dvc_symbol_log_probs_scratch_floats(long_row, 17, 1, 1, 1) == -1
+    refused(lib.dvc_symbol_log_probs(long_row, P, 8, P, P, P, P, P, None, 1, 1, 1, None), "scratch")
+    assert lib.dvc_symbol_log_probs_scratch_floats(lg(cs=1, classes=1000), 8, 1, 1, 1) == 0
 
 
 def test_python_surface_refuses_cpu_tensors_and_unknown_names():

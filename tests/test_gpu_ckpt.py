@@ -197,6 +197,9 @@ WGRAD = [
     (3, 1, (2,), 5, 1, 67, 2),
     (3, 1, (2,), 5, 67, 1, 2),
     (3, 1, (33,), 31, 70, 66, 1),
+    (3, 1, (32, 32), 40, 12, 36, 2),         # a staging wave's channels in one source each ...
+    (3, 1, (24, 40), 33, 12, 36, 2),         # ... and across two
+    (3, 1, (33,), 64, 200, 12, 1),
     (3, 2, (67,), 64, 32, 48, 1),
     (3, 2, (16,), 24, 25, 31, 2),
     (3, 2, (4,), 6, 1, 2, 1),
@@ -260,6 +263,46 @@ def test_weight_gradient_of_real_numbers(k, stride, cins, cout, h, w, batch, fmt
     assert torch.equal(again[0], gw) and torch.equal(again[1], gb)       # a fixed order of addition
 
 
+@pytest.mark.parametrize("k,stride,cin,cout,h,w,batch", [
+    (3, 1, 64, 64, 164, 256, 25),      # 8200 tiles over 256 workgroups: 33 for some (two slabs in time), 32 for most (one, and zeros)
+    (3, 1, 64, 33, 100, 260, 24),      # 56 or 57 tiles each on odd tile counts
+    (3, 1, 576, 576, 40, 160, 1),      # 81 blocks: four workgroups of 12 or 13 tiles each
+    (1, 1, 1024, 1024, 68, 92, 1),     # one workgroup per block: all 51 tiles
+    (7, 1, 32, 256, 132, 164, 2),      # 8 blocks, 12 or 13 tiles
+    (3, 2, 256, 512, 130, 132, 2),
+])
+def test_weight_gradient_of_long_sums(k, stride, cin, cout, h, w, batch):
+    """Many tiles per workgroup, several slabs in time, workgroups with one tile fewer than others: whole numbers, exact."""
+    from deepvideocodec_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(k + cin)
+    x = torch.randint(-1, 2, (batch, cin, h, w), generator=gen, device="cuda").float()
+    p = k // 2
+    ho, wo = (h + 2 * p - k) // stride + 1, (w + 2 * p - k) // stride + 1
+    g = torch.randint(-1, 2, (batch, cout, ho, wo), generator=gen, device="cuda").float()
+    assert batch * ho * wo < 1 << 24
+    gw, gb = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x), g, (cout, cin, k, k), stride, with_bias=True)
+    xp = F.pad(x, (p, p, p, p))
+    rows = g.double().transpose(0, 1).reshape(cout, -1)
+    for ky in range(k):
+        for kx in range(k):
+            cols = xp[:, :, ky:ky + (ho - 1) * stride + 1:stride, kx:kx + (wo - 1) * stride + 1:stride].double().transpose(0, 1).reshape(cin, -1)
+            assert torch.equal(gw[:, :, ky, kx].double(), rows @ cols.t().contiguous()), (ky, kx)
+    assert torch.equal(gb.double(), rows.sum(1))
+
+
+@pytest.mark.parametrize("e", [-60, -100, -118, 60, 100])
+def test_weight_gradient_of_very_small_and_large_gradients(e):
+    """A power of two on the gradient is one on the result, as long as nothing leaves the normal numbers."""
+    from deepvideocodec_amd import ops
+    gen = torch.Generator().manual_seed(8)
+    x = torch.randint(-15, 16, (1, 40, 12, 20), generator=gen).float()
+    g = torch.randint(-8, 9, (1, 36, 12, 20), generator=gen).float()
+    ck = ops.act_checkpoint(x.cuda())
+    a = ops.conv2d_wgrad_ckpt(ck, g.cuda(), (36, 40, 3, 3))
+    b = ops.conv2d_wgrad_ckpt(ck, (g * 2.0 ** e).cuda(), (36, 40, 3, 3))
+    assert torch.equal(a.double() * 2.0 ** e, b.double())
+
+
 def test_weight_gradient_keeps_all_bits_of_the_gradient():
     """One pixel: the result is a single product of a 24-bit gradient and a code, correctly rounded parts and all."""
     from deepvideocodec_amd import ops
@@ -320,6 +363,27 @@ def test_refusals_of_the_python_surface():
         ops.act_grad_signs(g, ops.act_signs(x), 0.1, False, tuple(g.shape))
     with pytest.raises(ValueError, match="shape"):
         ops.mul_act_grad_ckpt(g, ck, 0.1)
+    # destinations whose planes share memory
+    with pytest.raises(ValueError, match="overlapping"):
+        ops.act_restore(ck, out=torch.empty(1, 4, 8, 8, device="cuda").expand(2, 4, 8, 8))
+    with pytest.raises(ValueError, match="overlapping"):
+        ops.act_restore(ck, out=torch.empty(2, 1, 8, 8, device="cuda").expand(2, 4, 8, 8))
+    with pytest.raises(ValueError, match="overlapping"):
+        ops.mul_act_grad_ckpt(x, ck, 0.1, out=torch.empty(1, 4, 8, 8, device="cuda").expand(2, 4, 8, 8))
+    ops.act_restore(ck, out=torch.empty(4, 2, 8, 8, device="cuda").transpose(0, 1))      # interleaved samples do not
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    from deepvideocodec_amd import ops
+    x = torch.randn(2, 4, 8, 8, device="cuda")
+    ck = ops.act_checkpoint(x)
+    monkeypatch.setattr(ops, "_on_current_device", lambda t, name: (_ for _ in ()).throw(ValueError(f"{name}: other device")))
+    for call in (lambda: ops.act_checkpoint(x), lambda: ops.act_restore(ck), lambda: ops.act_signs(x),
+                 lambda: ops.act_grad_signs(x, torch.zeros(2, 4, 2, dtype=torch.int32, device="cuda"), 0.1, False, (2, 4, 8, 8)),
+                 lambda: ops.mul_act_grad_ckpt(x, ck, 0.1), lambda: ops.conv2d_wgrad_ckpt(ck, x, (4, 4, 3, 3)),
+                 lambda: ops.symbol_log_probs(x, torch.zeros(2, 2, 8, 8, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(ValueError, match="other device"):
+            call()
 
 
 def _lib_error():
@@ -477,3 +541,24 @@ def test_training_step_on_8_bit_storage(seeded_sd):
         assert set(res[storage][1]) == set(res["fp32"][1])
         assert all(bool(torch.isfinite(g).all()) for g in res[storage][1].values())
         assert held[storage] < held["fp32"], held
+
+
+def test_recompute_with_8_bit_storage(seeded_sd):
+    """Blocks that are recomputed in the backward pass store their operands in 8 bits while that runs: the same loss."""
+    from deepvideocodec_amd import train as TR
+    from deepvideocodec_amd.models import DMC
+    from deepvideocodec_amd.testing import synthetic_gop
+    frames = [f.cuda() for f in synthetic_gop(2, 64, 64, seed=3, batch=1)]
+    res = []
+    for recompute in (False, True):
+        net = DMC()
+        net.load_state_dict(seeded_sd)
+        net = net.cuda().train().set_act_storage("int8")
+        net.recompute = recompute
+        torch.manual_seed(5)
+        out = TR.RateDistortionLoss(lmbda=2048.0)(net(list(frames)), frames[1:])
+        out["loss"].backward()
+        res.append((out["loss"].item(), {n: p.grad for n, p in net.named_parameters() if p.grad is not None}))
+    (l0, g0), (l1, g1) = res
+    assert l0 == l1 and g0.keys() == g1.keys()
+    assert all(bool(torch.isfinite(g).all()) for g in g1.values())
