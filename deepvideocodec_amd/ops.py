@@ -642,14 +642,15 @@ def _ckpt_format(fmt: str) -> int:
 def _ckpt(ck: ActCheckpoint, name: str, device=None) -> DvcCkpt:
     if not isinstance(ck, ActCheckpoint):
         raise TypeError(f"{name}: expected an ActCheckpoint, got {type(ck)}")
-    fmt = _ckpt_format(ck.fmt)
-    n, c, h, w = ck.shape
-    if min(n, c, h, w) < 1:
+    codes, scales, (n, c, h, w), fmt = ck
+    fmt = _ckpt_format(fmt)
+    if n < 1 or c < 1 or h < 1 or w < 1:
         raise ValueError(f"{name}: empty shape {tuple(ck.shape)}")
-    _check_vec(ck.codes, n * c * _blocks(h, w) * 32, f"{name} codes", dtype=torch.uint8, device=device)
-    _check_vec(ck.scales, n * c * _blocks(h, w), f"{name} scales", dtype=torch.uint8, device=ck.codes.device)
-    _on_current_device(ck.codes, name)
-    return DvcCkpt(ck.codes.data_ptr(), ck.scales.data_ptr(), c, fmt)
+    blocks = n * c * ((h * w + 31) // 32)
+    _check_vec(codes, blocks * 32, f"{name} codes" if device is not None else name, dtype=torch.uint8, device=device)
+    _check_vec(scales, blocks, name, dtype=torch.uint8, device=codes.device)
+    _on_current_device(codes, name)
+    return DvcCkpt(codes.data_ptr(), scales.data_ptr(), c, fmt)
 
 
 def _distinct(t: Tensor, name: str):
@@ -676,8 +677,9 @@ def act_checkpoint(x: Tensor, slope: Optional[float] = None, fmt: str = "int8") 
     src = _src(x, "act_checkpoint x")
     _on_current_device(x, "act_checkpoint x")
     n, c, h, w = x.shape
-    codes = torch.empty((n, c, _blocks(h, w) * 32), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((n, c, _blocks(h, w)), dtype=torch.uint8, device=x.device)
+    blocks = (h * w + 31) // 32
+    codes = x.new_empty((n, c, blocks * 32), dtype=torch.uint8)
+    scales = x.new_empty((n, c, blocks), dtype=torch.uint8)
     check(_lib.load().dvc_act_checkpoint(C.byref(src), 0 if slope is None else 1,
                                          1.0 if slope is None else _slope(slope, "act_checkpoint"), code, codes.data_ptr(),
                                          scales.data_ptr(), n, h, w, _stream()), "dvc_act_checkpoint")
@@ -687,15 +689,17 @@ def act_checkpoint(x: Tensor, slope: Optional[float] = None, fmt: str = "int8") 
 def act_restore(ck: ActCheckpoint, out: Optional[Tensor] = None) -> Tensor:
     """The fp32 tensor a checkpoint stands for."""
     c = _ckpt(ck, "act_restore")
-    n, _, h, w = ck.shape
+    n, ch, h, w = ck.shape
     if out is None:
-        out = torch.empty(ck.shape, dtype=torch.float32, device=ck.codes.device)
-    elif tuple(out.shape) != tuple(ck.shape):
-        raise ValueError(f"act_restore: out shape {tuple(out.shape)} != {tuple(ck.shape)}")
-    dst = _dst(out)
-    _distinct(out, "act_restore out")
-    if out.device != ck.codes.device:
-        raise ValueError(f"act_restore: out on {out.device}, the checkpoint is on {ck.codes.device}")
+        out = ck.codes.new_empty(ck.shape, dtype=torch.float32)
+        dst = DvcDst(out.data_ptr(), ch * h * w, h * w)
+    else:
+        if tuple(out.shape) != tuple(ck.shape):
+            raise ValueError(f"act_restore: out shape {tuple(out.shape)} != {tuple(ck.shape)}")
+        dst = _dst(out)
+        _distinct(out, "act_restore out")
+        if out.device != ck.codes.device:
+            raise ValueError(f"act_restore: out on {out.device}, the checkpoint is on {ck.codes.device}")
     check(_lib.load().dvc_act_restore(C.byref(c), C.byref(dst), n, h, w, _stream()), "dvc_act_restore")
     return out
 
@@ -790,38 +794,34 @@ _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 def _logits(logits: Tensor, symbols: Tensor, name: str):
     """-> (DvcLogits or None without sites, n, groups, h, w, 2-D?)"""
-    for t, what in ((logits, "logits"), (symbols, "symbols")):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} {what}: expected a tensor, got {type(t)}")
-        if not t.is_cuda:
-            raise _lib.DvcError(f"{name} {what}: tensor is on {t.device}; the HIP path needs a GPU tensor (no CPU fallback)")
-    if logits.dtype not in _LOGIT_TYPES:
+    if not isinstance(logits, torch.Tensor) or not isinstance(symbols, torch.Tensor):
+        raise TypeError(f"{name}: expected tensors, got {type(logits)} and {type(symbols)}")
+    if not logits.is_cuda:
+        raise _lib.DvcError(f"{name} logits: tensor is on {logits.device}; the HIP path needs a GPU tensor (no CPU fallback)")
+    dtype = _LOGIT_TYPES.get(logits.dtype)
+    if dtype is None:
         raise TypeError(f"{name} logits: expected fp32, bf16 or fp16, got {logits.dtype}")
-    rows = logits.dim() == 2
-    if rows:
-        if symbols.dim() != 1:
-            raise ValueError(f"{name}: symbols {tuple(symbols.shape)} do not match logits {tuple(logits.shape)}")
-        n, groups, h, w = logits.size(0), 1, 1, 1
-        v, bs, cs = logits.size(1), logits.stride(0), logits.stride(1)
+    shape, site, strides = logits.shape, symbols.shape, logits.stride()
+    rows = len(shape) == 2
+    if rows and len(site) == 1:
+        (n, v), groups, h, w = shape, 1, 1, 1
+        match = site[0] == n
+    elif len(shape) == 4 and len(site) == 4:
+        n, groups, h, w = site
+        v = shape[1] // groups if groups else 0
+        match = shape[0] == n and shape[1] == groups * v and shape[2] == h and shape[3] == w
+        if w > 1 and strides[3] != 1 or h > 1 and strides[2] != w:
+            raise ValueError(f"{name} logits: rows must be contiguous (strides {strides})")
     else:
-        if logits.dim() != 4 or symbols.dim() != 4:
-            raise ValueError(f"{name}: expected logits (N, C * classes, h, w) with symbols (N, C, h, w), or (N, classes) with (N,), "
-                             f"got {tuple(logits.shape)} with {tuple(symbols.shape)}")
-        n, groups, h, w = symbols.shape
-        v = logits.size(1) // max(1, groups)
-        if logits.size(3) > 1 and logits.stride(3) != 1 or logits.size(2) > 1 and logits.stride(2) != logits.size(3):
-            raise ValueError(f"{name} logits: rows must be contiguous (strides {logits.stride()})")
-        bs, cs = logits.stride(0), logits.stride(1)
-    want = (n, v) if rows else (n, groups * v, h, w)
-    if tuple(logits.shape) != want or tuple(symbols.shape) != ((n,) if rows else (n, groups, h, w)) or groups < 1 or v < 1:
-        raise ValueError(f"{name}: symbols {tuple(symbols.shape)} do not match logits {tuple(logits.shape)}")
-    if logits.size(1) == 1:
-        cs = h * w
-    _check_vec(symbols, None, f"{name} symbols", dtype=torch.int32, device=logits.device)
-    _on_current_device(logits, f"{name} logits")
+        raise ValueError(f"{name}: expected logits (N, C * classes, h, w) with symbols (N, C, h, w), or (N, classes) with (N,), "
+                         f"got {tuple(shape)} with {tuple(site)}")
+    if not match or v < 1:
+        raise ValueError(f"{name}: symbols {tuple(site)} do not match logits {tuple(shape)}")
+    _check_vec(symbols, None, name, dtype=torch.int32, device=logits.device)
+    _on_current_device(logits, name)
     if n * h * w == 0:
         return None, n, groups, h, w, rows
-    return DvcLogits(logits.data_ptr(), bs, cs, groups, v, _LOGIT_TYPES[logits.dtype], 0), n, groups, h, w, rows
+    return DvcLogits(logits.data_ptr(), strides[0], strides[1] if shape[1] > 1 else h * w, groups, v, dtype, 0), n, groups, h, w, rows
 
 
 def symbol_log_probs(logits: Tensor, symbols: Tensor, top: int = 0) -> SymbolLogProbs:
@@ -833,24 +833,25 @@ def symbol_log_probs(logits: Tensor, symbols: Tensor, top: int = 0) -> SymbolLog
     fp32.  A symbol < 0 means "none here" (log probability 0); one past the last class gives NaN.  Classes that may not
     occur have logits of -inf; a site without any other has log probability -inf and entropy 0."""
     lg, n, groups, h, w, rows = _logits(logits, symbols, "symbol_log_probs")
-    dev = logits.device
     classes = logits.size(1) // groups
     top = int(top)
     if not 0 <= top <= min(_lib.MAX_TOP, classes):
         raise ValueError(f"symbol_log_probs: top={top} (0..{_lib.MAX_TOP}, at most the {classes} classes)")
     site = tuple(symbols.shape)
-    log_prob = torch.empty(site, dtype=torch.float32, device=dev)
-    entropy = torch.empty(site, dtype=torch.float32, device=dev)
-    stats = torch.empty((2, symbols.numel()), dtype=torch.float32, device=dev)
+    log_prob = symbols.new_empty(site, dtype=torch.float32)
+    entropy = torch.empty_like(log_prob)
+    stats = log_prob.new_empty((2, n * groups * h * w))
     tl = ts = None
     if top:
         shape = (n, top) if rows else (n, groups * top, h, w)
-        tl = torch.empty(shape, dtype=torch.float32, device=dev)
-        ts = torch.empty(shape, dtype=torch.int32, device=dev)
+        tl = log_prob.new_empty(shape)
+        ts = symbols.new_empty(shape)
     if lg is not None:
         lib = _lib.load()
-        nfl = check(lib.dvc_symbol_log_probs_scratch_floats(C.byref(lg), top, n, h, w), "dvc_symbol_log_probs_scratch_floats")
-        scratch = torch.empty(nfl, dtype=torch.float32, device=dev) if nfl else None
+        nfl = 0
+        if h * w == 1:      # only rows are ever cut into parts
+            nfl = check(lib.dvc_symbol_log_probs_scratch_floats(C.byref(lg), top, n, h, w), "dvc_symbol_log_probs_scratch_floats")
+        scratch = log_prob.new_empty(nfl) if nfl else None
         check(lib.dvc_symbol_log_probs(C.byref(lg), symbols.data_ptr(), top, log_prob.data_ptr(), entropy.data_ptr(),
                                        stats.data_ptr(), _ptr(tl), _ptr(ts), _ptr(scratch), n, h, w, _stream()), "dvc_symbol_log_probs")
     return SymbolLogProbs(log_prob, entropy, stats, tl, ts)
