@@ -23,7 +23,7 @@
 // next tile (loaded a tile ago) are decoded to bf16 / stored as fp32 while a tile is multiplied, and the loads of the one
 // after are issued.  A lane decodes four codes of a row (one dword).  The gradient stays fp32 in LDS (4 instead of 6
 // bytes) and is split when it is read, in the shadow of the matrix instructions; the bias gradient is summed by the lanes that
-// stage it.  Channel strides in LDS are odd multiples of 16 bytes: 16 lanes of a read (16 channels) fall on all 64 banks.
+// stage it.
 #pragma once
 #include <atomic>
 #include <type_traits>
@@ -167,13 +167,15 @@ struct Geo {
   static constexpr int ODD = TW + 8;                             // odd columns of a stride-2 row
   static constexpr int XROW = S == 1 ? 4 * XD : KS == 1 ? TW : TW + ODD;
   static_assert(XROW % 8 == 0, "rows on 16 bytes");
-  static constexpr int XUNITS = (IH * XROW / 8) | 1;             // 16-byte units per channel, odd
+  // bytes per channel: an odd multiple of what a lane reads at once (8 bytes for 3x3 stride 1, else 16), so that the lanes
+  // of a read -- channels -- fall on different banks
+  static constexpr int XREAD = KS == 3 && S == 1 ? 8 : 16, XSTR = ((IH * XROW * 2 / XREAD) | 1) * XREAD;
   static constexpr int GUNITS = (TH * TW / 4) | 1;
   static constexpr int XE = IH * XD, XSLOTS = (XE + 63) / 64;
   static constexpr int XPW = XCH / NS;                           // channels of x per staging wave
   static constexpr int GE = TH * TW / 4, GLOADS = GCH * GE / (64 * NS);      // 16-byte units of g per channel, per staging lane
   static_assert(GCH * GE % (64 * NS) == 0 && 64 % GE == 0, "gradient units deal out evenly, a channel's on adjacent lanes");
-  static constexpr int XBYTES = XCH * XUNITS * 16, BUF = XBYTES + GCH * GUNITS * 16;
+  static constexpr int XBYTES = XCH * XSTR, BUF = XBYTES + GCH * GUNITS * 16;
   static constexpr int LDS_BYTES = 2 * BUF;
   static_assert(LDS_BYTES <= 160 * 1024, "LDS");
   static constexpr int STEPS = TH * TW / 16;                     // row pieces of 16 pixels per tile
@@ -334,7 +336,7 @@ struct Stager {
           v.y = mask[j] > 3 ? v.y : mask[j] > 2 ? v.y & 0xffffu : 0u;
         }
         if (64 * (j + 1) <= G::XE || e < G::XE) {
-          char* const row = buf + ((XPW * sw + c) * G::XUNITS * 8 + iy * G::XROW) * 2;
+          char* const row = buf + (XPW * sw + c) * G::XSTR + iy * G::XROW * 2;
           if constexpr (S == 1) {
             *reinterpret_cast<uint2*>(row + 8 * q) = v;
           } else {
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
 
   const int ga = G::XBYTES + (mt * 32 + l32) * G::GUNITS * 16 + half * 32;
-  const int xa = (ct * 32 + l32) * G::XUNITS * 16 + half * 16;
+  const int xa = (ct * 32 + l32) * G::XSTR + half * 16;
   constexpr int ROWS = KS == 7 ? 1 : KS;            // staged rows a row piece meets in this wave
   constexpr int STEPS = G::STEPS / KG;              // row pieces per tile in this wave
 
