@@ -45,7 +45,8 @@ class _Conv2d(torch.autograd.Function):
         else:
             # 8-bit storage: the activated sources as checkpoints (for the weight gradient and, by their sign bits, the
             # input activation's derivative), the output activation's derivative as one bit per value
-            ctx.kept, tensors = _keep(srcs, in_slope, storage, ctx.needs_input_grad[0] or in_slope is not None)
+            need = ctx.needs_input_grad
+            ctx.kept, tensors = _keep(srcs, in_slope, storage, need[0] or in_slope is not None and any(need[13:]))
             ctx.save_for_backward(weight, ops.act_signs(out) if out_slope is not None else None, *tensors)
         return out
 

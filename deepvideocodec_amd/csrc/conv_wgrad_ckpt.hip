@@ -8,50 +8,50 @@ int launch_aligned(int ks, int stride, const Args& a, const Plan& p, hipStream_t
 
 namespace {
 
-// gW[co][ci][tap] = sum over slabs of partial[slab][tap][co][ci], gB[co] likewise over splits (indices past the weight's).  A block
-// takes 64 results; each of its WAVES waves adds every WAVES-th slab, with the loads of four slabs in flight, and the sums are
-// added in a fixed order.  16 waves for many slabs (256 of a 64 x 64 3x3 layer: 9 us, 20 with four waves and one load after
-// the other), 4 for few.
-template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int slabs, int nsplit, int taps, int cout, int cin,
-                                                                 int cout_pad, int cin_pad, const float* bias_partial, float* gb) {
-  __shared__ float part[WAVES][64];
-  const long long total = (long long)cout * taps * cin;
-  const long long total_all = total + (gb != nullptr ? cout : 0);
-  const int lane = threadIdx.x & 63, kg = threadIdx.x >> 6;
-  for (long long i0 = blockIdx.x * 64LL; i0 < total_all; i0 += (long long)gridDim.x * 64) {
-    const long long i = i0 + lane;
-    const float* p = nullptr;
-    long long step = 0, dst = -1;
-    int count = slabs;
-    if (i < total) {
-      const unsigned r = (unsigned)i, ci = r % (unsigned)cin, q = r / (unsigned)cin;      // (a weight has below 2^31 elements)
-      const unsigned tap = q % (unsigned)taps, co = q / (unsigned)taps;
-      p = partial + ((long long)tap * cout_pad + co) * cin_pad + ci;
-      step = (long long)taps * cout_pad * cin_pad;
-      dst = ((long long)co * cin + ci) * taps + tap;
-    } else if (i < total_all) {
-      p = bias_partial + (i - total);
-      step = cout_pad;
-      count = nsplit;
+// gW[co][ci][tap] = sum over slabs of partial[slab][tap][co][ci], gB[co] likewise over splits (units past the weight's).  A lane
+// takes four adjacent input channels (rows of a slab are padded to 32), a block UNITS such units; each of its GROUPS groups of
+// lanes adds every GROUPS-th slab, with the loads of four slabs in flight, and the sums are added in a fixed order.
+__device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+
+template <int UNITS, int GROUPS>
+__global__ __launch_bounds__(UNITS * GROUPS) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int slabs, int nsplit, int taps,
+                                                                       int cout, int cin, int cout_pad, int cin_pad,
+                                                                       const float* bias_partial, float* gb) {
+  __shared__ float4 part[GROUPS][UNITS];
+  const unsigned cin4 = (unsigned)(cin + 3) / 4, units = (unsigned)cout * (unsigned)taps * cin4;
+  const unsigned all = units + (gb != nullptr ? (unsigned)(cout + 3) / 4 : 0u);
+  const int lane = threadIdx.x % UNITS, kg = threadIdx.x / UNITS;
+  for (unsigned i0 = blockIdx.x * (unsigned)UNITS; i0 < all; i0 += gridDim.x * (unsigned)UNITS) {
+    const unsigned i = i0 + lane;
+    const unsigned ci = i % cin4 * 4, q = i / cin4, tap = q % (unsigned)taps, co = q / (unsigned)taps;
+    const bool weight = i < units;
+    const float* const p = weight ? partial + ((long long)tap * cout_pad + co) * cin_pad + ci : bias_partial + 4ll * (i - units);
+    const long long step = weight ? (long long)taps * cout_pad * cin_pad : cout_pad;
+    const int count = i < all ? (weight ? slabs : nsplit) : 0;
+    auto at = [&](int k) { return *reinterpret_cast<const float4*>(p + k * step); };
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    int k = kg;
+    for (; k + 3 * GROUPS < count; k += 4 * GROUPS) {
+      const float4 v0 = at(k), v1 = at(k + GROUPS), v2 = at(k + 2 * GROUPS), v3 = at(k + 3 * GROUPS);
+      s = add4(s, add4(add4(v0, v1), add4(v2, v3)));
     }
-    float s = 0.f;
-    if (p != nullptr) {
-      int k = kg;
-      for (; k + 3 * WAVES < count; k += 4 * WAVES) {
-        const float v0 = p[k * step], v1 = p[(k + WAVES) * step], v2 = p[(k + 2 * WAVES) * step], v3 = p[(k + 3 * WAVES) * step];
-        s += (v0 + v1) + (v2 + v3);
-      }
-      for (; k < count; k += WAVES) s += p[k * step];
-    }
+    for (; k < count; k += GROUPS) s = add4(s, at(k));
     part[kg][lane] = s;
     __syncthreads();
-    if (kg == 0 && p != nullptr) {
-      float v = part[0][lane];
+    if (kg == 0 && i < all) {
+      float4 v = part[0][lane];
+#pragma unroll 5      // (all 63 of the widest form would not fit the registers of 16 waves)
+      for (int w = 1; w < GROUPS; ++w) v = add4(v, part[w][lane]);
+      const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 1; k < WAVES; ++k) v += part[k][lane];
-      if (dst >= 0) gw[dst] = v;
-      else gb[i - total] = v;
+      for (int j = 0; j < 4; ++j) {
+        if (weight) {
+          if ((int)ci + j < cin) gw[((long long)co * cin + ci + j) * taps + tap] = r[j];
+        } else {
+          const int c = (int)(4 * (i - units)) + j;
+          if (c < cout) gb[c] = r[j];
+        }
+      }
     }
     __syncthreads();
   }
@@ -128,6 +128,7 @@ extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t
   int cin;
   if (int rc = check_srcs(srcs, n_src, &cin, who)) return rc;
   DVC_REQUIRE(grad_out != nullptr && scratch != nullptr && grad_weight != nullptr, "%s: null pointer", who);
+  DVC_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "%s: scratch must start on 16 bytes", who);
   Plan p;
   if (int rc = make_plan(out_channels, cin, ksize, stride, batch, in_h, in_w, &p, who)) return rc;
   Args a{};
@@ -163,12 +164,16 @@ extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t
   const bool aligned = in_w % 4 == 0 && p.wo % 4 == 0 && reinterpret_cast<uintptr_t>(grad_out) % 16 == 0 &&
                        4LL * out_channels * p.ho * p.wo < (1LL << 31);
   if (int rc = aligned ? launch_aligned(ksize, stride, a, p, st) : launch_any(ksize, stride, a, p, st)) return rc;
-  const long long total = (long long)out_channels * cin * p.taps + out_channels;
-  const dim3 grid((unsigned)((total + 63) / 64 < 16384 ? (total + 63) / 64 : 16384));
-#define REDUCE(WAVES) hipLaunchKernelGGL(wgrad_ckpt_reduce_kernel<WAVES>, grid, dim3(64 * WAVES), 0, st, scratch, grad_weight, p.slabs, p.nsplit, \
-                                         p.taps, out_channels, cin, p.cout_pad, p.cin_pad, a.bias_partial, grad_bias)
-  if (p.slabs >= 64) REDUCE(16);
-  else REDUCE(4);
+  const long long units = (long long)out_channels * p.taps * ((cin + 3) / 4) + (out_channels + 3) / 4;
+  // Blocks of 64 units by 16 groups (64->64 3x3 in 256 slabs: 8 us, 16 by 64 10); where those are fewer than half the CUs, 16 by
+  // 64 (3->64 3x3 in 1024 slabs: 42 us in 10 blocks, 18 in 37); of few slabs 64 by 4.
+#define REDUCE(UNITS, GROUPS)                                                                                                        \
+  hipLaunchKernelGGL((wgrad_ckpt_reduce_kernel<UNITS, GROUPS>), dim3((unsigned)((units + UNITS - 1) / UNITS < 16384 ? (units + UNITS - 1) / UNITS : 16384)), \
+                     dim3(UNITS * GROUPS), 0, st, scratch, grad_weight, p.slabs, p.nsplit, p.taps, out_channels, cin, p.cout_pad, p.cin_pad, \
+                     a.bias_partial, grad_bias)
+  if (p.slabs < 64) REDUCE(64, 4);
+  else if (units < 64 * 128) REDUCE(16, 64);
+  else REDUCE(64, 16);
 #undef REDUCE
   return dvc::check_launch("wgrad_ckpt_reduce_kernel");
 }

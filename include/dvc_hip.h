@@ -378,8 +378,7 @@ int dvc_sq_err_backward(const DvcSrc* a, const DvcSrc* b, const float* grad_sse,
  * to NaN.  A code is a byte: bit 7 = "not greater than zero" (set for zero as well, so that an activation's derivative
  * is read off the code alone, also where the magnitude rounded to zero), the low seven bits the magnitude, rounded
  * to nearest even (in the topmost binade down where up would be 2^128).  The last block of a plane is filled with code 128.  codes are contiguous (batch, channels,
- * blocks * 32), scales (batch, channels, blocks), blocks = ceil(h*w / 32); codes start on 16 bytes, scales on 4 (a
- * scale is read as a byte; what matters is that both belong to one tensor of that shape).
+ * blocks * 32), scales (batch, channels, blocks), blocks = ceil(h*w / 32); codes start on 16 bytes.
  */
 #define DVC_CKPT_INT8 0
 #define DVC_CKPT_E4M3 1
@@ -403,7 +402,7 @@ int dvc_act_grad_signs(const DvcSrc* grad, const uint32_t* signs, float slope, i
 int dvc_mul_act_grad_ckpt(const DvcSrc* grad, const DvcCkpt* x, float slope, const DvcSrc* plus, const DvcDst* out,
                           int32_t batch, int32_t h, int32_t w, void* stream);
 /* dvc_conv2d_wgrad with the sources given by checkpoints of their activated values (all of one format).
- * Deterministic.  The products are exact: a code times its power of two is a bf16 number, and the gradient is split
+ * Deterministic; scratch starts on 16 bytes.  The products are exact: a code times its power of two is a bf16 number, and the gradient is split
  * into three bf16 parts that add up to it; sums are fp32.  (A block that restores to NaN, or a gradient that is not
  * finite, reaches every weight it takes part in as NaN.) */
 int64_t dvc_conv2d_wgrad_ckpt_scratch_floats(int32_t cout, int32_t cin, int32_t ksize, int32_t stride,

@@ -69,6 +69,7 @@ def test_weight_gradient_refusals():
     refused(call(one, grad=None), "null")
     refused(call(one, scratch=None), "null")
     refused(call(one, h=0), "dims")
+    refused(call(one, scratch=P + 4), "16 bytes")
     refused(call((DvcCkpt * 1)(DvcCkpt(P + 1, P, 3, 0))), "16 bytes")
     refused(call((DvcCkpt * 2)(DvcCkpt(P, P, 3, 0), DvcCkpt(P, P, 3, 1)), n=2), "format")
     assert lib.dvc_conv2d_wgrad_ckpt_scratch_floats(4, 3, 5, 1, 1, 8, 8) == -1

@@ -171,6 +171,66 @@ def test_masks_and_values_that_are_not_finite(dtype, rows):
     assert grad[3].tolist() == [0, 0, 0, 0, 0, 0]      # certain: no gradient
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_rows_of_every_kind(dtype):
+    """Rows that are cut over workgroups: one value throughout, rising, falling, nothing allowed, one class allowed, a NaN, an
+    infinity, the best classes in one place or at the ends."""
+    from deepvideocodec_amd import ops
+    v = 50003
+    g = torch.Generator().manual_seed(11)
+    noise = torch.randn(v, generator=g)
+    rows = [torch.full((v,), 1.5), torch.arange(v) / 512.0, -torch.arange(v) / 512.0, torch.full((v,), NEG), torch.full((v,), NEG),
+            noise.clone(), noise.clone(), noise.clone(), noise.clone(), torch.full((v,), torch.finfo(dtype).min)]
+    rows[4][31007] = -3.0
+    rows[5][40000] = float("nan")
+    rows[6][123] = float("inf")
+    rows[7][20000:20040] += 20
+    rows[8][[0, 1, 2, v - 1, v - 2, v - 3]] += 30
+    x = torch.stack(rows).to(dtype)
+    sym = torch.tensor([5, v - 1, 0, 7, 31007, 3, 123, 20001, v - 1, 9], dtype=torch.int32)
+    given, ent, tl, ts, lp, p = definition(x, sym, 16)
+    for n in (10, 1):                     # in nine parts, in twelve
+        r = ops.symbol_log_probs(x[:n].cuda(), sym[:n].cuda(), 16)
+        tol = (2 * 104 + 16 + -(-v // 64) + 64) * 2.0 ** -23
+        same(r.log_prob, given[:n], tol + given[:n].abs().nan_to_num(0, 0, 0) * 2.0 ** -23)
+        same(r.entropy, ent[:n], tol * (2 + ent[:n].nan_to_num(0)))
+        assert torch.equal(r.top_symbol.cpu(), ts[:n])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ties_in_long_rows(dtype):
+    """Of tens of thousands of equally good classes the lowest, over all parts of a row."""
+    from deepvideocodec_amd import ops
+    x = torch.randint(0, 3, (9, 70000), generator=torch.Generator().manual_seed(13)).float()
+    want = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :16].to(torch.int32)
+    r = ops.symbol_log_probs(x.to(dtype).cuda(), torch.zeros(9, dtype=torch.int32).cuda(), 16)
+    assert torch.equal(r.top_symbol.cpu(), want)
+
+
+def test_two_streams_at_once():
+    """The same calls on two streams side by side: workspaces are each call's own."""
+    from deepvideocodec_amd import ops
+    g = torch.Generator().manual_seed(12)
+    xs = [torch.randn(3, 60000, generator=g).cuda() for _ in range(2)]
+    s = torch.randint(0, 60000, (3,), generator=g, dtype=torch.int32).cuda()
+    acts = [ops.act_checkpoint(torch.randn(4, 64, 64, 64, generator=g).cuda()) for _ in range(2)]
+    grads = [torch.randn(4, 64, 64, 64, generator=g).cuda() for _ in range(2)]
+    work = lambda i: [*ops.symbol_log_probs(xs[i], s, 8), *ops.conv2d_wgrad_ckpt(acts[i], grads[i], (64, 64, 3, 3), with_bias=True)]
+    want = [[t.clone() for t in work(i)] for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            for a, b in zip(out, want[i]):
+                assert torch.equal(a, b)
+
+
 def test_symbols_outside_the_classes():
     from deepvideocodec_amd import autograd as A, ops
     x = torch.randn(4, 10, generator=torch.Generator().manual_seed(0)).cuda().requires_grad_()
