@@ -615,18 +615,141 @@ __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Lo
       }
 }
 
+// ---------------------------------------------------------------- many short rows
+// A wave of its own is far too much for a row of a few classes.  Here a wave takes 64 / L rows at once: their logits go
+// through LDS (read as one run of 16-byte vectors where rows follow each other), then L lanes share a row, `per` adjacent
+// classes each.  `per` is odd, so the lanes' addresses lane * per + k fall on different banks.  Rows are evenly spaced,
+// `pitch` elements apart.
+constexpr int kShortClasses = 256;        // longest row of this form
+constexpr int kShortPer = 32;             // classes of a lane
+
+struct ShortRows {
+  const void* p;
+  long long pitch;
+  int classes, lanes, per;
+  unsigned inv;                           // ceil(2^32 / classes): i / classes = umulhi(i, inv) for i < 2^16 (classes >= 2)
+  __device__ __forceinline__ unsigned row_of(unsigned i) const { return classes == 1 ? i : __umulhi(i, inv); }
+};
+
+template <int DT, int TOP>
+__global__ __launch_bounds__(64) void symbol_short_rows_kernel(ShortRows l, const int* symbols, int top, float* log_prob, float* entropy,
+                                                               float* stats, float* top_lp, int* top_sym, int sites) {
+  typedef typename Elem<DT>::type T;
+  constexpr int N = Vec<DT>::N;
+  extern __shared__ float tile[];         // 64 * per
+  const int lane = threadIdx.x, rows = 64 / l.lanes, site0 = (int)blockIdx.x * rows;
+  const int count = sites - site0 < rows ? sites - site0 : rows;
+  const T* const base = static_cast<const T*>(l.p) + (long long)site0 * l.pitch;
+  const int row_floats = l.lanes * l.per, total = count * l.classes;
+  auto put1 = [&](int i) {
+    const int r = (int)l.row_of((unsigned)i), c = i - r * l.classes;
+    tile[r * row_floats + c] = Elem<DT>::up(base[(long long)r * l.pitch + c]);
+  };
+  if (l.pitch == l.classes) {
+    const RowPart rp = row_part<DT>(base, total);
+    if (lane < rp.head + total - rp.tail0) put1(lane < rp.head ? lane : rp.tail0 + lane - rp.head);
+    const uint4* const body = reinterpret_cast<const uint4*>(base + rp.head);
+    constexpr int U = 4;                  // vectors in flight per lane
+    for (int j = lane; j < rp.body; j += U * 64) {
+      Vec<DT> q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * 64 < rp.body) q[u].q = body[j + u * 64];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * 64 < rp.body) {
+          const int i = rp.head + (j + u * 64) * N;
+          const int r = (int)l.row_of((unsigned)i);
+          int c = i - r * l.classes;
+          float* at = tile + r * row_floats + c;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            *at = Elem<DT>::up(q[u].e[e]);
+            ++at;
+            if (++c == l.classes) { c = 0; at += row_floats - l.classes; }
+          }
+        }
+    }
+  } else {
+    for (int i = lane; i < total; i += 64) put1(i);
+  }
+  const int r = lane / l.lanes, part = lane - r * l.lanes;
+  const bool live = r < count;
+  const int sym = live && part == 0 ? symbols[site0 + r] : -1;
+  __syncthreads();
+
+  Stat st;
+  st.clear();
+  ThreadList<TOP> list;
+  list.clear();
+  if (live) {
+    const float* const x = tile + lane * l.per;
+    const int v0 = part * l.per, mine = l.classes - v0 < l.per ? l.classes - v0 : l.per;
+    auto take = [&](float f, int k) {
+      if constexpr (TOP > 0) {
+        const unsigned key = order_key(f);
+        if (key > list.key[TOP - 1]) list.insert(key, v0 + k);
+      }
+    };
+    constexpr int U = 8;
+    int k = 0;
+    for (; k + U <= mine; k += U) {
+      float f[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) f[u] = x[k + u];
+      add_many<U>(&st, f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) take(f[u], k + u);
+    }
+    for (; k < mine; ++k) {
+      const float f = x[k];
+      add_many<1>(&st, &f);
+      take(f, k);
+    }
+  }
+  // a row's first lane collects: the lane o further on holds higher classes, so equal keys go behind
+  for (int o = 1; o < l.lanes; o <<= 1) {
+    st.join(__shfl_down(st.m, o, 64), __shfl_down(st.s, o, 64), __shfl_down(st.t, o, 64));
+    if constexpr (TOP > 0) {
+      unsigned key[TOP];
+      int cls[TOP];
+#pragma unroll
+      for (int j = 0; j < TOP; ++j) { key[j] = (unsigned)__shfl_down((int)list.key[j], o, 64); cls[j] = __shfl_down(list.cls[j], o, 64); }
+#pragma unroll
+      for (int j = 0; j < TOP; ++j)
+        if (key[j] > list.key[TOP - 1]) list.insert(key[j], cls[j]);
+    }
+  }
+  if (!live || part != 0) return;
+  float log_s, h;
+  finish(st, &log_s, &h);
+  const int site = site0 + r;
+  const float given_x = sym >= 0 && sym < l.classes ? tile[r * row_floats + sym] : 0.f;
+  log_prob[site] = given_log_p(sym, l.classes, given_x, st.m, log_s);
+  entropy[site] = h;
+  stats[site] = st.m;
+  stats[(long long)sites + site] = log_s;
+  if constexpr (TOP > 0)
+#pragma unroll
+    for (int j = 0; j < TOP; ++j)
+      if (j < top) {
+        top_lp[(long long)site * top + j] = log_p(key_value(list.key[j]), st.m, log_s);
+        top_sym[(long long)site * top + j] = list.cls[j];
+      }
+}
+
 // ---------------------------------------------------------------- gradient: one read, one write
 struct SiteGrad {
   float m, log_s, h, a, b;
   int sym;
-  __device__ __forceinline__ void load(const Logits& l, const int* symbols, const float* stats, const float* entropy, const float* g_lp,
+  __device__ __forceinline__ void load(int classes, const int* symbols, const float* stats, const float* entropy, const float* g_lp,
                                        const float* g_h, long long i, long long sites) {
     sym = symbols[i];
     m = stats[i];
     m = m == NEG_INF ? 0.f : m;
     log_s = stats[sites + i];
     h = entropy[i];
-    a = g_lp != nullptr && sym >= 0 ? (sym < l.classes ? g_lp[i] : __uint_as_float(0x7fc00000u)) : 0.f;
+    a = g_lp != nullptr && sym >= 0 ? (sym < classes ? g_lp[i] : __uint_as_float(0x7fc00000u)) : 0.f;
     b = g_h != nullptr ? g_h[i] : 0.f;
   }
   __device__ __forceinline__ float of(float x, int v) const {
@@ -635,6 +758,58 @@ struct SiteGrad {
     return v == sym ? d + a : d;
   }
 };
+
+// Rows of up to kFlatClasses: a wave takes `rows` (at most 64) of them, their statistics wait in LDS, and the lanes go over
+// the rows' logits as one run (2097152 x 37 fp32 125 us, 2455 with a workgroup per row; 262144 x 1000 bf16 204 / 393).
+constexpr int kFlatClasses = 1024;
+
+template <int DT>
+__global__ __launch_bounds__(64) void symbol_short_rows_backward_kernel(ShortRows l, const int* symbols, const float* stats,
+                                                                        const float* entropy, const float* g_lp, const float* g_h,
+                                                                        typename Elem<DT>::type* grad, int sites, int rows) {
+  typedef typename Elem<DT>::type T;
+  constexpr int N = Vec<DT>::N;
+  __shared__ SiteGrad of_row[64];
+  const int lane = threadIdx.x, site0 = (int)blockIdx.x * rows;
+  const int count = sites - site0 < rows ? sites - site0 : rows;
+  const T* const base = static_cast<const T*>(l.p) + (long long)site0 * l.pitch;
+  T* const out = grad + (long long)site0 * l.classes;
+  const int total = count * l.classes;
+  if (lane < count) of_row[lane].load(l.classes, symbols, stats, entropy, g_lp, g_h, site0 + lane, sites);
+  __syncthreads();
+  auto one = [&](int i) {
+    const int r = (int)l.row_of((unsigned)i), c = i - r * l.classes;
+    out[i] = Elem<DT>::down(of_row[r].of(Elem<DT>::up(base[(long long)r * l.pitch + c]), c));
+  };
+  if (l.pitch == l.classes && ((reinterpret_cast<uintptr_t>(base) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
+    const RowPart rp = row_part<DT>(base, total);
+    if (lane < rp.head + total - rp.tail0) one(lane < rp.head ? lane : rp.tail0 + lane - rp.head);
+    const uint4* const body = reinterpret_cast<const uint4*>(base + rp.head);
+    uint4* const to = reinterpret_cast<uint4*>(out + rp.head);
+    constexpr int U = 4;                  // vectors in flight per lane
+    for (int j = lane; j < rp.body; j += U * 64) {
+      Vec<DT> q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * 64 < rp.body) q[u].q = body[j + u * 64];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * 64 < rp.body) {
+          const int i = rp.head + (j + u * 64) * N;
+          int r = (int)l.row_of((unsigned)i), c = i - r * l.classes;
+          SiteGrad sg = of_row[r];
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            q[u].e[e] = Elem<DT>::down(sg.of(Elem<DT>::up(q[u].e[e]), c));
+            if (e < N - 1 && ++c == l.classes) { c = 0; sg = of_row[++r]; }
+          }
+          to[j + u * 64] = q[u].q;
+        }
+    }
+  } else {
+    for (int i = lane; i < total; i += 64) one(i);
+  }
+}
 
 constexpr int kRowVecs = 4;      // vectors per thread of the row form
 
@@ -649,7 +824,7 @@ __global__ __launch_bounds__(256) void symbol_rows_backward_kernel(Logits l, con
   const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes;
   T* const out = grad + (long long)site * l.classes;
   SiteGrad sg;
-  sg.load(l, symbols, stats, entropy, g_lp, g_h, site, sites);
+  sg.load(l.classes, symbols, stats, entropy, g_lp, g_h, site, sites);
   RowPart rp = row_part<DT>(row, l.classes);
   const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;   // one vector grid for both
   const int j0 = chunk * 256 * kRowVecs + threadIdx.x;
@@ -699,7 +874,7 @@ __global__ __launch_bounds__(256) void symbol_planes_backward_kernel(Logits l, c
   const T* const row = static_cast<const T*>(l.p) + (long long)n * l.bs + (long long)g * l.classes * l.cs + p;
   T* const out = grad + ng * l.classes * hw + p;
   SiteGrad sg;
-  sg.load(l, symbols, stats, entropy, g_lp, g_h, i, sites);
+  sg.load(l.classes, symbols, stats, entropy, g_lp, g_h, i, sites);
   const int v0 = (int)chunk * kPlaneClasses;
   T q[kPlaneClasses];
 #pragma unroll
@@ -722,9 +897,24 @@ int check_logits(const DvcLogits* l, int batch, int h, int w, const char* who) {
 }
 inline Logits mk(const DvcLogits* l) { return Logits{l->ptr, l->batch_stride, l->class_stride, l->groups, l->classes}; }
 
+// (a launch has below 2^32 threads)
+inline bool fits(long long blocks, int threads) { return blocks * threads < (1ll << 32); }
+
 // The classes of a site are adjacent: one pixel per plane and unit class stride (groups follow each other).
 inline bool is_rows(const DvcLogits* l, int h, int w) {
   return h == 1 && w == 1 && (l->class_stride == 1 || (l->classes == 1 && l->groups == 1));
+}
+
+// Rows one pitch apart, whatever their group: what the short forms take.
+inline bool evenly_spaced(const DvcLogits* l, int batch) {
+  return l->groups == 1 || batch == 1 || l->batch_stride == (int64_t)l->groups * l->classes;
+}
+inline ShortRows short_rows(const DvcLogits* l, int batch) {
+  ShortRows r{l->ptr, l->groups == 1 && batch > 1 ? l->batch_stride : l->classes, l->classes, 1, 0,
+              l->classes == 1 ? 0u : (unsigned)(((1ull << 32) + l->classes - 1) / l->classes)};
+  while (r.lanes * kShortPer < r.classes) r.lanes *= 2;
+  r.per = (r.classes + r.lanes - 1) / r.lanes | 1;
+  return r;
 }
 
 // Into how many parts a row is cut: while the rows alone give fewer than 512 workgroups (two per CU), as long as a part
@@ -743,14 +933,32 @@ int launch_forward(const DvcLogits* l, const int32_t* symbols, int top, float* l
   const unsigned hw = (unsigned)((long long)h * w);
   const long long sites = (long long)batch * l->groups * hw;
   if (is_rows(l, h, w)) {
+    // Many short rows share waves (below 8192 rows both forms are the call's own latency)
+    if (l->classes <= kShortClasses && sites >= 8192 && evenly_spaced(l, batch)) {
+      const ShortRows r = short_rows(l, batch);
+      const int rows = 64 / r.lanes;
+      const dim3 grid((unsigned)((sites + rows - 1) / rows));
+      DVC_REQUIRE(fits((sites + rows - 1) / rows, 64), "dvc_symbol_log_probs: too many sites");
+#define SHORT(TOP) hipLaunchKernelGGL((symbol_short_rows_kernel<DT, TOP>), grid, dim3(64), 64 * r.per * sizeof(float), st, r, symbols, top, \
+                                      log_prob, entropy, stats, top_lp, top_sym, (int)sites)
+      if (top == 0) SHORT(0);
+      else if (top == 1) SHORT(1);
+      else if (top <= 4) SHORT(4);
+      else if (top <= 8) SHORT(8);
+      else SHORT(16);
+#undef SHORT
+      return dvc::check_launch("symbol_short_rows_kernel");
+    }
     // a wave per row while a row is at most a few vectors per lane
     if (l->classes <= 1024) {
+      DVC_REQUIRE(fits((sites + 3) / 4, 256), "dvc_symbol_log_probs: too many sites");
       hipLaunchKernelGGL((symbol_rows_kernel<DT, 64>), dim3((unsigned)((sites + 3) / 4)), dim3(256), 0, st, mk(l), symbols, top, log_prob,
                          entropy, stats, top_lp, top_sym, (int)sites, 1, Parts{});
       return dvc::check_launch("symbol_rows_kernel");
     }
     const int nparts = row_parts(l, batch, h, w);
     const long long units = sites * nparts;
+    DVC_REQUIRE(fits(units, 256), "dvc_symbol_log_probs: too many sites");
     Parts parts{};
     if (nparts > 1) {
       DVC_REQUIRE(scratch != nullptr, "dvc_symbol_log_probs: null scratch");
@@ -765,7 +973,7 @@ int launch_forward(const DvcLogits* l, const int32_t* symbols, int top, float* l
     return dvc::check_launch("symbol_rows_join_kernel");
   }
   const long long waves = (sites + 63) / 64;
-  DVC_REQUIRE(waves < (1LL << 31), "dvc_symbol_log_probs: too many sites");
+  DVC_REQUIRE(fits((sites + 255) / 256, 256), "dvc_symbol_log_probs: too many sites");
 #define PLANES(TOP, SL) hipLaunchKernelGGL((symbol_planes_kernel<DT, TOP, SL>), dim3((unsigned)((sites + (SL == 1 ? 255 : 63)) / (SL == 1 ? 256 : 64))), \
                                            dim3(SL == 1 ? 256 : 64 * SL), 0, st, mk(l), symbols, top, log_prob, entropy, stats, top_lp,      \
                                            top_sym, sites, hw)
@@ -793,16 +1001,25 @@ int launch_backward(const DvcLogits* l, const int32_t* symbols, const float* sta
   typedef typename Elem<DT>::type T;
   const unsigned hw = (unsigned)((long long)h * w);
   const long long sites = (long long)batch * l->groups * hw;
+  if (is_rows(l, h, w) && l->classes <= kFlatClasses && evenly_spaced(l, batch)) {
+    // up to 4096 logits a wave, fewer while that gives below 2048 waves
+    int rows = 64;
+    while (rows > 1 && ((long long)rows * l->classes > 4096 || sites < 2048ll * rows)) rows /= 2;
+    DVC_REQUIRE(fits((sites + rows - 1) / rows, 64), "%s: too many sites", who);
+    hipLaunchKernelGGL(symbol_short_rows_backward_kernel<DT>, dim3((unsigned)((sites + rows - 1) / rows)), dim3(64), 0, st,
+                       short_rows(l, batch), symbols, stats, entropy, g_lp, g_h, static_cast<T*>(grad), (int)sites, rows);
+    return dvc::check_launch("symbol_short_rows_backward_kernel");
+  }
   if (is_rows(l, h, w)) {
     const int per = 256 * kRowVecs * Vec<DT>::N;
     const long long chunks = (l->classes + per - 1) / per;
-    DVC_REQUIRE(sites * chunks < (1LL << 31), "%s: too many sites", who);
+    DVC_REQUIRE(fits(sites * chunks, 256), "%s: too many sites", who);
     hipLaunchKernelGGL(symbol_rows_backward_kernel<DT>, dim3((unsigned)(sites * chunks)), dim3(256), 0, st, mk(l), symbols, stats, entropy,
                        g_lp, g_h, static_cast<T*>(grad), (int)sites, (int)chunks);
     return dvc::check_launch("symbol_rows_backward_kernel");
   }
   const long long chunks = (l->classes + kPlaneClasses - 1) / kPlaneClasses, blocks = (sites + 255) / 256;
-  DVC_REQUIRE(blocks * chunks < (1LL << 31), "%s: too many sites", who);
+  DVC_REQUIRE(fits(blocks * chunks, 256), "%s: too many sites", who);
   hipLaunchKernelGGL(symbol_planes_backward_kernel<DT>, dim3((unsigned)(blocks * chunks)), dim3(256), 0, st, mk(l), symbols, stats, entropy,
                      g_lp, g_h, static_cast<T*>(grad), sites, hw, (unsigned)chunks);
   return dvc::check_launch("symbol_planes_backward_kernel");

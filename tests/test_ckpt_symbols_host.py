@@ -103,6 +103,12 @@ def test_symbol_refusals():
     assert lib.dvc_symbol_log_probs_scratch_floats(long_row, 17, 1, 1, 1) == -1
     refused(lib.dvc_symbol_log_probs(long_row, P, 8, P, P, P, P, P, None, 1, 1, 1, None), "scratch")
     assert lib.dvc_symbol_log_probs_scratch_floats(lg(cs=1, classes=1000), 8, 1, 1, 1) == 0
+    # more threads than a launch has
+    refused(lib.dvc_symbol_log_probs(lg(cs=1, classes=1000), P, 0, P, P, P, None, None, None, 1 << 27, 1, 1, None), "too many")
+    refused(lib.dvc_symbol_log_probs(lg(cs=1, classes=5000), P, 0, P, P, P, None, None, None, 1 << 25, 1, 1, None), "too many")
+    refused(lib.dvc_symbol_log_probs_backward(lg(cs=1, classes=5000), P, P, P, P, P, P, 1 << 25, 1, 1, None), "too many")
+    refused(lib.dvc_symbol_log_probs(lg(cs=1 << 27, classes=4), P, 0, P, P, P, None, None, None, 64, 1 << 13, 1 << 14, None), "too many")
+    refused(lib.dvc_symbol_log_probs_backward(lg(cs=1 << 27, classes=400), P, P, P, P, P, P, 64, 1 << 13, 1 << 14, None), "too many")
 
 
 def test_python_surface_refuses_cpu_tensors_and_unknown_names():

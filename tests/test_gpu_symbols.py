@@ -198,6 +198,43 @@ def test_long_rows_of_every_kind(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", (1, 2, 3, 7, 31, 64, 65, 100, 128, 129, 255, 256))
+def test_many_short_rows(classes, dtype):
+    """Rows that share a wave: values, alternatives and gradient; masked rows, a NaN, an infinity; rows that follow each other on
+    16 bytes, off them, and rows apart."""
+    from deepvideocodec_amd import ops
+    n = 8192 + 37
+    logits, symbols, g = inputs(0, classes, n, 0, 0, dtype, 5)
+    logits[100] = NEG
+    logits[8191] = torch.finfo(dtype).min
+    logits[8200, classes // 2] = float("nan")
+    logits[n - 1, classes - 1] = float("inf")
+    symbols[[0, 64, n - 2]] = classes
+    top = min(classes, 8)
+    given, ent, tl, ts, lp, p = definition(logits, symbols, top)
+    tol = step(classes, lp)
+    gl, gh = (torch.randn(n, generator=g) for _ in range(2))
+    a, b = torch.where(symbols < 0, 0.0, gl.double())[:, None], gh.double()[:, None]
+    pr, lpr = p.view(n, classes), lp.view(n, classes)
+    want = -pr * a - b * torch.where(pr == 0, 0.0, pr * (lpr + ent[:, None])) + a * (torch.arange(classes)[None] == symbols[:, None])
+    want[symbols == classes] = float("nan")
+    bound = tol * (a.abs() + b.abs() * (2 + 2 * ent[:, None].nan_to_num(0))) + want.abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).smallest_normal
+    flat = torch.zeros(n * classes + 1, dtype=dtype).cuda()
+    wide = torch.zeros(n, classes + 3, dtype=dtype).cuda()
+    for x in (logits.cuda(), flat[1:].view(n, classes), wide[:, 1:1 + classes]):
+        x.copy_(logits)
+        for t in {0, 1, min(3, top), top, min(classes, 16)}:
+            r = ops.symbol_log_probs(x, symbols.cuda(), t)
+            same(r.log_prob, given, tol + given.abs().nan_to_num(0, 0, 0) * 2.0 ** -23)
+            same(r.entropy, ent, tol * (2 + ent.nan_to_num(0)))
+            if 0 < t <= top:
+                assert torch.equal(r.top_symbol.cpu(), ts[:, :t])
+                same(r.top_log_prob, tl[:, :t], tol + tl[:, :t].abs().nan_to_num(0, 0, 0) * 2.0 ** -23)
+        got = ops.symbol_log_probs_backward(x, symbols.cuda(), r.stats, r.entropy, gl.cuda(), gh.cuda())
+        same(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_ties_in_long_rows(dtype):
     """Of tens of thousands of equally good classes the lowest, over all parts of a row."""
     from deepvideocodec_amd import ops
