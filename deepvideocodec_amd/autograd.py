@@ -10,6 +10,7 @@ csrc/conv_wgrad.hip.
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -497,6 +498,7 @@ class _SymbolLogProbs(torch.autograd.Function):
         return r.log_prob, r.entropy, r.top_log_prob, r.top_symbol
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_lp, g_h, _top_lp, _top_sym):
         if g_lp is None and g_h is None:
             return None, None, None

@@ -562,3 +562,40 @@ def test_recompute_with_8_bit_storage(seeded_sd):
     (l0, g0), (l1, g1) = res
     assert l0 == l1 and g0.keys() == g1.keys()
     assert all(bool(torch.isfinite(g).all()) for g in g1.values())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_past_two_to_the_31_values(fmt):
+    """More than 2^31 values and 2^33 bytes: the last sample's checkpoint, signs, adjoints and weight gradient are its own."""
+    from deepvideocodec_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(21)
+    x = torch.empty((33, 64, 1024, 1024), device="cuda").uniform_(-1, 1, generator=g)
+    assert x.numel() > 1 << 31
+    ck, one = ops.act_checkpoint(x, 0.1, fmt), ops.act_checkpoint(x[-1:], 0.1, fmt)
+    assert torch.equal(ck.codes[-1:], one.codes) and torch.equal(ck.scales[-1:], one.scales)
+    signs = ops.act_signs(x)
+    assert torch.equal(signs[-1:], ops.act_signs(x[-1:]))
+    assert torch.equal(ops.act_grad_signs(x, signs, 0.5, False, x.shape)[-1:], ops.act_grad_signs(x[-1:], signs[-1:], 0.5, False, (1, *x.shape[1:])))
+    assert torch.equal(ops.mul_act_grad_ckpt(x, ck, 0.5)[-1:], ops.mul_act_grad_ckpt(x[-1:], one, 0.5))
+    out = ops.act_restore(ck, out=x)
+    assert out is x and torch.equal(x[-1:], ops.act_restore(one))
+    # whole numbers below 2^24: every order of the sums gives the same
+    x.random_(-1, 2, generator=g)
+    grad = torch.zeros((33, 64, 1024, 1024), device="cuda")
+    grad[-1].random_(-1, 2, generator=g)
+    gw, gb = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x, None, fmt), grad, (64, 64, 3, 3), with_bias=True)
+    ow, ob = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x[-1:], None, fmt), grad[-1:].contiguous(), (64, 64, 3, 3), with_bias=True)
+    assert torch.equal(gw, ow) and torch.equal(gb, ob) and float(gw.abs().max()) > 1000
+
+
+def test_weight_gradient_of_one_huge_sample():
+    """A sample's gradient of more than 2^31 bytes, against a product in 64 bits."""
+    from deepvideocodec_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(22)
+    h, w = 3001, 3000
+    x = torch.empty((1, 64, h, w), device="cuda").random_(-1, 2, generator=g)
+    grad = torch.empty((1, 64, h, w), device="cuda").random_(-1, 2, generator=g)
+    assert grad.numel() * 4 > 1 << 31 and h * w < 1 << 24         # (whole numbers: exact sums)
+    got = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x), grad, (64, 64, 1, 1)).view(64, 64)
+    want = grad.view(64, -1).double() @ x.view(64, -1).double().t()
+    assert torch.equal(got.double(), want)

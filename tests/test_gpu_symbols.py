@@ -234,6 +234,58 @@ def test_many_short_rows(classes, dtype):
         same(got, want, bound)
 
 
+def test_one_row_for_all_sites():
+    """Expanded logits (no stride between rows), also where rows share waves."""
+    from deepvideocodec_amd import ops
+    for classes in (37, 300):
+        g = torch.Generator().manual_seed(15)
+        x = torch.randn(1, classes, generator=g).cuda().expand(9000, classes)
+        sym = torch.randint(-1, classes, (9000,), generator=g, dtype=torch.int32).cuda()
+        gl = torch.randn(9000, generator=g).cuda()
+        res = [ops.symbol_log_probs(t, sym, 3) for t in (x, x.contiguous())]
+        grads = [ops.symbol_log_probs_backward(t, sym, r.stats, r.entropy, gl, gl) for t, r in zip((x, x.contiguous()), res)]
+        for a, b in zip((*res[0], grads[0]), (*res[1], grads[1])):
+            assert torch.equal(a, b)
+
+
+def test_no_second_derivative():
+    from deepvideocodec_amd import autograd as A
+    x = torch.randn(4, 9, generator=torch.Generator().manual_seed(16)).cuda().requires_grad_()
+    lp = A.symbol_log_probs(x, torch.zeros(4, dtype=torch.int32).cuda())[0]
+    (grad,) = torch.autograd.grad(lp.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        grad.sum().backward()
+    lp = A.symbol_log_probs(x, torch.zeros(4, dtype=torch.int32).cuda())[0]
+    (grad,) = torch.autograd.grad((lp * lp).sum(), x, create_graph=True)      # (the seed depends on x)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grad.sum().backward()
+
+
+@pytest.mark.parametrize("n,groups,classes,h,w", [(70001, 0, 32768, 0, 0), (35000003, 0, 64, 0, 0), (2200001, 0, 1000, 0, 0), (9, 4, 64, 1024, 1024)])
+def test_past_two_to_the_31_logits(n, groups, classes, h, w):
+    """The last sites of a tensor of more than 2^31 logits are those of the last sites alone."""
+    from deepvideocodec_amd import ops
+    rows = groups == 0
+    g = torch.Generator(device="cuda").manual_seed(17)
+    x = torch.empty((n, classes) if rows else (n, groups * classes, h, w), dtype=torch.bfloat16, device="cuda").uniform_(-3, 3, generator=g)
+    assert x.numel() > 1 << 31
+    sym = torch.randint(0, classes, (n,) if rows else (n, groups, h, w), generator=g, dtype=torch.int32, device="cuda")
+    gl = torch.empty(sym.shape, device="cuda").uniform_(-1, 1, generator=g)
+    r = ops.symbol_log_probs(x, sym, 2)
+    got = ops.symbol_log_probs_backward(x, sym, r.stats, r.entropy, gl, gl)
+    last = lambda t: (t[-40:] if rows else t[-1:, :, -2:]).cpu()
+    given, ent, tl, ts, lp, p = definition(last(x), last(sym), 2)
+    tol = step(classes, lp)
+    same(last(r.log_prob), given, tol)
+    same(last(r.entropy), ent, tol * (2 + ent))
+    assert torch.equal(last(r.top_symbol), ts)
+    site = lambda t: last(t).double().view(lp.size(0), lp.size(1), 1, *lp.shape[3:])
+    a, en = site(gl), ent.view(lp.size(0), lp.size(1), 1, *lp.shape[3:])
+    want = -p * (a + a * (lp + en)) + a * (torch.arange(classes).view(1, 1, -1, 1, 1) == site(sym))
+    bound = tol * a.abs() * (3 + 2 * en) + want.abs() * 2.0 ** -8 + torch.finfo(torch.bfloat16).smallest_normal
+    same(last(got), want.view(last(x).shape), bound.expand(want.shape).reshape(last(x).shape))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ties_in_long_rows(dtype):
     """Of tens of thousands of equally good classes the lowest, over all parts of a row."""
