@@ -458,6 +458,38 @@ def test_side_stream_and_replayed_graph():
             assert torch.equal(a, b)
 
 
+def test_forward_and_backward_in_a_replayed_graph():
+    """The autograd form as a whole under capture, of a leaf that no eager graph holds."""
+    from deepvideocodec_amd import autograd as A
+    g = torch.Generator().manual_seed(14)
+    sym = torch.randint(-1, 50, (3, 2, 4, 5), generator=g, dtype=torch.int32).cuda()
+    gl, gh = (torch.randn(sym.shape, generator=g).cuda() for _ in range(2))
+
+    def passes(x):
+        r = A.symbol_log_probs(x, sym)
+        (grad,) = torch.autograd.grad((r[0], r[1]), x, (gl, gh))
+        return r[0].detach(), r[1].detach(), grad
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes(torch.randn(3, 100, 4, 5, generator=g).cuda().requires_grad_())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    leaf = torch.zeros(3, 100, 4, 5).cuda().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = passes(leaf)
+    for _ in range(4):
+        fresh = torch.randn(leaf.shape, generator=g).cuda()
+        with torch.no_grad():
+            leaf.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, passes(fresh.requires_grad_())):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_categorical_rate_behind_checkpointed_layers(fmt):
     """As used together: a stack of convolutions whose tape is 8-bit, logits for a small alphabet, bits as the loss.
