@@ -527,7 +527,39 @@ struct ThreadList {
   }
 };
 
-template <int DT, int TOP, int SL>
+// The same for 16-bit logits of at most 65536 classes: key and class share a word (higher class, smaller word), all words
+// differ, and taking one is a minimum and a maximum per place -- no compares to carry, no order of arrival (bf16 planes 32 x 4 x 64
+// classes x 64 x 64: 32 us with 4 alternatives, 60 with 16, the list above 42 and 98; a single alternative is cheaper above).
+constexpr int kPackedClasses = 65536;
+template <int DT> __device__ __forceinline__ unsigned order_key16(typename Elem<DT>::type v) {
+  const unsigned b = __builtin_bit_cast(unsigned short, v);
+  constexpr unsigned INF = DT == DVC_BF16 ? 0x7f80u : 0x7c00u;
+  const unsigned k = (b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u;
+  return (b & 0x7fffu) > INF ? 0xffffu : b == 0x8000u ? 0x8000u : k;
+}
+template <int DT> __device__ __forceinline__ float key16_value(unsigned k) {
+  return Elem<DT>::up(__builtin_bit_cast(typename Elem<DT>::type, (unsigned short)((k & 0x8000u) ? k ^ 0x8000u : ~k)));
+}
+template <int TOP>
+struct PackedList {
+  unsigned word[TOP > 0 ? TOP : 1];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < TOP; ++j) word[j] = 0;
+  }
+  __device__ __forceinline__ void insert(unsigned w) {
+#pragma unroll
+    for (int j = 0; j < TOP; ++j) {
+      const unsigned up = w > word[j] ? w : word[j];
+      w = w > word[j] ? word[j] : w;
+      word[j] = up;
+    }
+  }
+  static __device__ __forceinline__ unsigned pack(unsigned key, int c) { return key << 16 | (0xffffu - (unsigned)c); }
+  __device__ __forceinline__ int cls(int j) const { return (int)(0xffffu - (word[j] & 0xffffu)); }
+};
+
+template <int DT, int TOP, int SL, bool PACK>
 __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Logits l, const int* symbols, int top, float* log_prob,
                                                                               float* entropy, float* stats, float* top_lp,
                                                                               int* top_sym, long long sites, unsigned hw) {
@@ -535,7 +567,7 @@ __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Lo
   constexpr int SITES = SL == 1 ? 256 : 64;
   __shared__ float part[SL > 1 ? SL * 3 * 64 : 1];
   __shared__ unsigned keys[SL > 1 && TOP > 0 ? SL * TOP * 64 : 1];
-  __shared__ int classes_of[SL > 1 && TOP > 0 ? SL * TOP * 64 : 1];
+  __shared__ int classes_of[SL > 1 && TOP > 0 && !PACK ? SL * TOP * 64 : 1];
   const int slot = threadIdx.x % SITES;
   const int slice = SL == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x / SITES));
   const long long i = (long long)blockIdx.x * SITES + slot;
@@ -550,11 +582,15 @@ __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Lo
 
   Stat st;
   st.clear();
-  ThreadList<TOP> list;
+  ThreadList<PACK ? 0 : TOP> list;
+  PackedList<PACK ? TOP : 0> packed;
   list.clear();
+  packed.clear();
   float last = NEG_INF;
-  auto take = [&](float x, int v) {
-    if constexpr (TOP > 0) {
+  auto take = [&](T raw, float x, int v) {
+    if constexpr (TOP > 0 && PACK) {
+      packed.insert(packed.pack(order_key16<DT>(raw), v));
+    } else if constexpr (TOP > 0) {
       if (v - v0 < TOP || !(x <= last)) {      // (a NaN, or behind one, compares false: the keys decide)
         list.insert(order_key(x), v);
         last = list.key[TOP - 1] != 0 ? key_value(list.key[TOP - 1]) : NEG_INF;
@@ -564,17 +600,22 @@ __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Lo
   constexpr int U = 8;
   int v = v0;
   for (; v + U <= v1; v += U) {
+    T raw[U];
     float x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = Elem<DT>::up(row[(long long)(v + u) * l.cs]);
+    for (int u = 0; u < U; ++u) {
+      raw[u] = row[(long long)(v + u) * l.cs];
+      x[u] = Elem<DT>::up(raw[u]);
+    }
     add_many<U>(&st, x);
 #pragma unroll
-    for (int u = 0; u < U; ++u) take(x[u], v + u);
+    for (int u = 0; u < U; ++u) take(raw[u], x[u], v + u);
   }
   for (; v < v1; ++v) {
-    const float x = Elem<DT>::up(row[(long long)v * l.cs]);
+    const T raw = row[(long long)v * l.cs];
+    const float x = Elem<DT>::up(raw);
     add_many<1>(&st, &x);
-    take(x, v);
+    take(raw, x, v);
   }
 
   if constexpr (SL > 1) {
@@ -584,8 +625,12 @@ __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Lo
     if constexpr (TOP > 0)
 #pragma unroll
       for (int j = 0; j < TOP; ++j) {
-        keys[(slice * TOP + j) * 64 + slot] = list.key[j];
-        classes_of[(slice * TOP + j) * 64 + slot] = list.cls[j];
+        if constexpr (PACK) {
+          keys[(slice * TOP + j) * 64 + slot] = packed.word[j];
+        } else {
+          keys[(slice * TOP + j) * 64 + slot] = list.key[j];
+          classes_of[(slice * TOP + j) * 64 + slot] = list.cls[j];
+        }
       }
     __syncthreads();
     if (slice != 0) return;
@@ -594,7 +639,8 @@ __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Lo
       if constexpr (TOP > 0)
         for (int j = 0; j < TOP; ++j) {
           const unsigned k = keys[(s * TOP + j) * 64 + slot];
-          if (k > list.key[TOP - 1]) list.insert(k, classes_of[(s * TOP + j) * 64 + slot]);
+          if constexpr (PACK) packed.insert(k);
+          else if (k > list.key[TOP - 1]) list.insert(k, classes_of[(s * TOP + j) * 64 + slot]);
         }
     }
   }
@@ -610,8 +656,13 @@ __global__ __launch_bounds__(SL == 16 ? 1024 : 256) void symbol_planes_kernel(Lo
     for (int j = 0; j < TOP; ++j)
       if (j < top) {
         const long long at = (ng * top + j) * hw + p;
-        top_lp[at] = log_p(key_value(list.key[j]), st.m, log_s);
-        top_sym[at] = list.cls[j];
+        if constexpr (PACK) {
+          top_lp[at] = log_p(key16_value<DT>(packed.word[j] >> 16), st.m, log_s);
+          top_sym[at] = packed.cls(j);
+        } else {
+          top_lp[at] = log_p(key_value(list.key[j]), st.m, log_s);
+          top_sym[at] = list.cls[j];
+        }
       }
 }
 
@@ -636,6 +687,7 @@ __global__ __launch_bounds__(64) void symbol_short_rows_kernel(ShortRows l, cons
                                                                float* stats, float* top_lp, int* top_sym, int sites) {
   typedef typename Elem<DT>::type T;
   constexpr int N = Vec<DT>::N;
+  constexpr bool PACK = DT != DVC_F32 && TOP > 1;    // (at most kShortClasses classes)
   extern __shared__ float tile[];         // 64 * per
   const int lane = threadIdx.x, rows = 64 / l.lanes, site0 = (int)blockIdx.x * rows;
   const int count = sites - site0 < rows ? sites - site0 : rows;
@@ -680,13 +732,17 @@ __global__ __launch_bounds__(64) void symbol_short_rows_kernel(ShortRows l, cons
 
   Stat st;
   st.clear();
-  ThreadList<TOP> list;
+  ThreadList<PACK ? 0 : TOP> list;
+  PackedList<PACK ? TOP : 0> packed;
   list.clear();
+  packed.clear();
   if (live) {
     const float* const x = tile + lane * l.per;
     const int v0 = part * l.per, mine = l.classes - v0 < l.per ? l.classes - v0 : l.per;
     auto take = [&](float f, int k) {
-      if constexpr (TOP > 0) {
+      if constexpr (TOP > 0 && PACK) {
+        packed.insert(packed.pack(order_key16<DT>(Elem<DT>::down(f)), v0 + k));      // (exact: it was of that type)
+      } else if constexpr (TOP > 0) {
         const unsigned key = order_key(f);
         if (key > list.key[TOP - 1]) list.insert(key, v0 + k);
       }
@@ -710,7 +766,13 @@ __global__ __launch_bounds__(64) void symbol_short_rows_kernel(ShortRows l, cons
   // a row's first lane collects: the lane o further on holds higher classes, so equal keys go behind
   for (int o = 1; o < l.lanes; o <<= 1) {
     st.join(__shfl_down(st.m, o, 64), __shfl_down(st.s, o, 64), __shfl_down(st.t, o, 64));
-    if constexpr (TOP > 0) {
+    if constexpr (TOP > 0 && PACK) {
+      unsigned word[TOP];
+#pragma unroll
+      for (int j = 0; j < TOP; ++j) word[j] = (unsigned)__shfl_down((int)packed.word[j], o, 64);
+#pragma unroll
+      for (int j = 0; j < TOP; ++j) packed.insert(word[j]);
+    } else if constexpr (TOP > 0) {
       unsigned key[TOP];
       int cls[TOP];
 #pragma unroll
@@ -733,8 +795,14 @@ __global__ __launch_bounds__(64) void symbol_short_rows_kernel(ShortRows l, cons
 #pragma unroll
     for (int j = 0; j < TOP; ++j)
       if (j < top) {
-        top_lp[(long long)site * top + j] = log_p(key_value(list.key[j]), st.m, log_s);
-        top_sym[(long long)site * top + j] = list.cls[j];
+        const long long at = (long long)site * top + j;
+        if constexpr (PACK) {
+          top_lp[at] = log_p(key16_value<DT>(packed.word[j] >> 16), st.m, log_s);
+          top_sym[at] = packed.cls(j);
+        } else {
+          top_lp[at] = log_p(key_value(list.key[j]), st.m, log_s);
+          top_sym[at] = list.cls[j];
+        }
       }
 }
 
@@ -974,16 +1042,21 @@ int launch_forward(const DvcLogits* l, const int32_t* symbols, int top, float* l
   }
   const long long waves = (sites + 63) / 64;
   DVC_REQUIRE(fits((sites + 255) / 256, 256), "dvc_symbol_log_probs: too many sites");
-#define PLANES(TOP, SL) hipLaunchKernelGGL((symbol_planes_kernel<DT, TOP, SL>), dim3((unsigned)((sites + (SL == 1 ? 255 : 63)) / (SL == 1 ? 256 : 64))), \
-                                           dim3(SL == 1 ? 256 : 64 * SL), 0, st, mk(l), symbols, top, log_prob, entropy, stats, top_lp,      \
-                                           top_sym, sites, hw)
+#define PLANES(TOP, SL, PACK)                                                                                                          \
+  hipLaunchKernelGGL((symbol_planes_kernel<DT, TOP, SL, PACK>), dim3((unsigned)((sites + (SL == 1 ? 255 : 63)) / (SL == 1 ? 256 : 64))), \
+                     dim3(SL == 1 ? 256 : 64 * SL), 0, st, mk(l), symbols, top, log_prob, entropy, stats, top_lp, top_sym, sites, hw)
   // Cut the classes while the sites alone give fewer than eight waves per CU and a range keeps eight classes; the joining
   // lists of 16 ranges fit LDS up to 4 alternatives
-#define SLICES(TOP)                                                                        \
-  do {                                                                                     \
-    if (TOP <= 4 && waves < 512 && l->classes >= 128) PLANES(TOP, (TOP <= 4 ? 16 : 4));    \
-    else if (waves < 2048 && l->classes >= 32) PLANES(TOP, 4);                             \
-    else PLANES(TOP, 1);                                                                   \
+#define SLICES_OF(TOP, PACK)                                                                     \
+  do {                                                                                           \
+    if (TOP <= 4 && waves < 512 && l->classes >= 128) PLANES(TOP, (TOP <= 4 ? 16 : 4), PACK);    \
+    else if (waves < 2048 && l->classes >= 32) PLANES(TOP, 4, PACK);                             \
+    else PLANES(TOP, 1, PACK);                                                                   \
+  } while (0)
+#define SLICES(TOP)                                                                              \
+  do {                                                                                           \
+    if (TOP > 1 && DT != DVC_F32 && l->classes <= kPackedClasses) SLICES_OF(TOP, (TOP > 1 && DT != DVC_F32)); \
+    else SLICES_OF(TOP, false);                                                                  \
   } while (0)
   if (top == 0) SLICES(0);
   else if (top == 1) SLICES(1);
@@ -991,6 +1064,7 @@ int launch_forward(const DvcLogits* l, const int32_t* symbols, int top, float* l
   else if (top <= 8) SLICES(8);
   else SLICES(16);
 #undef SLICES
+#undef SLICES_OF
 #undef PLANES
   return dvc::check_launch("symbol_planes_kernel");
 }

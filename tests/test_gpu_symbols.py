@@ -234,6 +234,29 @@ def test_many_short_rows(classes, dtype):
         same(got, want, bound)
 
 
+@pytest.mark.parametrize("classes", [40, 65536, 65537, 70001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_alternatives_in_planes_of_very_many_classes(dtype, classes):
+    """16-bit planes around 65536 classes: ties, signed zeros, an infinity, a NaN, minus infinity throughout."""
+    from deepvideocodec_amd import ops
+    g = torch.Generator().manual_seed(18)
+    x = torch.randint(-3, 4, (1, classes, 2, 3), generator=g).to(dtype)
+    x = torch.where((x == 0) & (torch.rand(x.shape, generator=g) < 0.5), -x, x)
+    x[0, -1, 0, 0] = float("inf")
+    x[0, classes // 2, 0, 1] = float("nan")
+    x[0, :, 0, 2] = NEG
+    x[0, :, 1, 0] = torch.where(torch.arange(classes) == classes - 2, 0.0, float("nan")).to(dtype)
+    x[0, :, 1, 1] = -x[0, :, 1, 1].abs()
+    sym = torch.randint(0, classes, (1, 1, 2, 3), generator=g, dtype=torch.int32)
+    for top in (1, 3, 7, 16):
+        given, ent, tl, ts, lp, p = definition(x, sym, top)
+        r = ops.symbol_log_probs(x.cuda(), sym.cuda(), top)
+        assert torch.equal(r.top_symbol.cpu(), ts)
+        tol = (2 * 104 + 16 + classes + 64) * 2.0 ** -23
+        same(r.log_prob, given, tol)
+        same(r.top_log_prob, tl, tol)
+
+
 def test_one_row_for_all_sites():
     """Expanded logits (no stride between rows), also where rows share waves."""
     from deepvideocodec_amd import ops
