@@ -119,10 +119,55 @@ __device__ __forceinline__ unsigned nth_of_16(unsigned v, int nth, int lane) {
   const int ge = 1 + not_below<15>(v);
   return wave_max(lane < 16 && ge >= nth ? v : 0);
 }
+// the same over lanes 0..31: a row's own sixteen and the other row's
+template <int R>
+__device__ __forceinline__ int other_not_below(unsigned o, unsigned v) {
+  const unsigned r = (unsigned)__builtin_amdgcn_mov_dpp((int)o, 0x120 + R, 0xF, 0xF, true);
+  if constexpr (R > 1) return (r >= v ? 1 : 0) + other_not_below<R - 1>(o, v);
+  else return r >= v ? 1 : 0;
+}
+__device__ __forceinline__ unsigned nth_of_32(unsigned v, int nth, int lane) {
+  const unsigned o = (unsigned)__shfl_xor((int)v, 16, 64);
+  const int ge = 1 + not_below<15>(v) + (o >= v ? 1 : 0) + other_not_below<15>(o, v);
+  return wave_max(lane < 32 && ge >= nth ? v : 0);
+}
 
+template <int CTRL> __device__ __forceinline__ unsigned max_with(unsigned v) {
+  const unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+  return v > o ? v : o;
+}
+// a bound for the `top` best of a wave whose lanes hold the maxima of pairs: over the pairs, or over pairs of them
+__device__ __forceinline__ unsigned group_bound(unsigned pair, int top, int lane) {
+  if (top > 8) return nth_of_32((unsigned)__shfl((int)pair, 2 * (lane & 31), 64), top, lane);
+  return nth_of_16((unsigned)__shfl((int)max_with<0x4E>(pair), 4 * (lane & 15), 64), top, lane);
+}
+template <int CTRL> __device__ __forceinline__ float lane_of(float v) {
+  return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float read_lane(float v, int l) { return __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); }
+__device__ __forceinline__ float wave_maxf(float v) {         // uniform results; the same swaps as in wave_max
+  v = fmaxf(v, lane_of<0xB1>(v));
+  v = fmaxf(v, lane_of<0x4E>(v));
+  v = fmaxf(v, lane_of<0x141>(v));
+  v = fmaxf(v, lane_of<0x140>(v));
+  return fmaxf(fmaxf(read_lane(v, 0), read_lane(v, 16)), fmaxf(read_lane(v, 32), read_lane(v, 48)));
+}
+__device__ __forceinline__ float wave_sumf(float v) {
+  v += lane_of<0xB1>(v);
+  v += lane_of<0x4E>(v);
+  v += lane_of<0x141>(v);
+  v += lane_of<0x140>(v);
+  return (read_lane(v, 0) + read_lane(v, 16)) + (read_lane(v, 32) + read_lane(v, 48));
+}
+
+// the 64 lanes' statistics in one: the maximum first, so that each lane is rescaled once (262144 rows of 1000 bf16: 143 us;
+// joined in pairs, with six shuffles of three values and twelve exponentials, 177)
 __device__ __forceinline__ void wave_join(Stat* st) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) st->join(__shfl_xor(st->m, o, 64), __shfl_xor(st->s, o, 64), __shfl_xor(st->t, o, 64));
+  const float mm = wave_maxf(st->m);
+  const float a = st->m == mm ? 1.f : __expf(st->m - mm), d = st->m == mm ? 0.f : fmaxf(st->m - mm, kFloor);
+  st->t = wave_sumf(a * (st->t + st->s * d));
+  st->s = wave_sumf(a * st->s);
+  st->m = mm;
 }
 
 // A wave's list of the best classes so far: lane j < top holds the j-th (key, class), best first.  An empty place has
@@ -187,9 +232,10 @@ __device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(
 // latency of its own loads: 25 us) and a second kernel joins the parts.
 //
 // The alternatives cost no second pass: a lane's running maximum is the largest of its own classes.  The lanes form
-// sixteen groups; the `top`-th largest of the groups' maxima (top <= 16) is a lower bound for the top-th best class, and only
-// lanes whose maximum reaches it can hold one (of random classes about 16 ln 2 reach the bound for top 8).  Those few lanes
-// go over their own classes again (in cache) and put what reaches the bound into a small pool, whose members are then
+// sixteen groups (32 above 8 alternatives: the least of 16 maxima is a poor bound, 262144 rows of 1000 bf16 with 16
+// alternatives 585 us, 336 with 32); the `top`-th largest of the groups' maxima (top <= 16) is a lower bound for the top-th best class, and only lanes whose maximum reaches it can hold one (of random classes about 16 ln 2 reach the
+// bound for top 8).  The classes of those few lanes are gone over again (in cache; shared out over the wave: 4096 rows of
+// 32768 bf16 with 8 alternatives 62 us, 82 with each lane on its own), and what reaches the bound goes into a small pool, whose members are then
 // placed by counting (inserting them one by one into a sorted list, which remains for pools that overflow, was half the
 // time of a short row).
 template <int DT> struct Vec {
@@ -320,28 +366,28 @@ __global__ __launch_bounds__(256) void symbol_rows_kernel(Logits l, const int* s
   if constexpr (WAVES > 1) {
     if (lane == 0) { part[wave * 3] = all.m; part[wave * 3 + 1] = all.s; part[wave * 3 + 2] = all.t; }
   }
-  // the groups' maxima: four lanes each where the row is a wave, sixteen where it is a workgroup
+  // the groups' maxima: four (two) lanes each where the row is a wave, sixteen (eight) where it is a workgroup
   unsigned bound = 0;
+  const bool many = top > 8;
   if (top > 0) {
-    unsigned k = best, o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0xB1, 0xF, 0xF, true);
-    k = k > o ? k : o;
-    o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x4E, 0xF, 0xF, true);
-    k = k > o ? k : o;
+    unsigned k = max_with<0xB1>(best);
     if constexpr (WAVES > 1) {
-      o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x141, 0xF, 0xF, true);
-      k = k > o ? k : o;
-      o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x140, 0xF, 0xF, true);
-      k = k > o ? k : o;
-      if ((lane & 15) == 0) keys[wave * 4 + (lane >> 4)] = k;
+      k = max_with<0x141>(max_with<0x4E>(k));
+      if (many) {
+        if ((lane & 7) == 0) keys[wave * 8 + (lane >> 3)] = k;
+      } else {
+        k = max_with<0x140>(k);
+        if ((lane & 15) == 0) keys[wave * 4 + (lane >> 4)] = k;
+      }
     } else {
-      bound = nth_of_16((unsigned)__shfl((int)k, 4 * (lane & 15), 64), top, lane);
+      bound = group_bound(k, top, lane);
     }
   }
   if constexpr (WAVES > 1) {
     __syncthreads();
     all.clear();
     for (int w = 0; w < WAVES; ++w) all.join(part[w * 3], part[w * 3 + 1], part[w * 3 + 2]);
-    if (top > 0) bound = nth_of_16(keys[lane & 15], top, lane);
+    if (top > 0) bound = many ? nth_of_32(keys[lane & 31], top, lane) : nth_of_16(keys[lane & 15], top, lane);
   }
   float log_s, h;
   finish(all, &log_s, &h);
@@ -349,12 +395,18 @@ __global__ __launch_bounds__(256) void symbol_rows_kernel(Logits l, const int* s
   if (top > 0) {
     const bool in = best >= bound && best != 0;      // (fewer groups than `top` with a class: bound 0, all look)
     const unsigned end_k = in && has_end ? order_key(end_x) : 0;
-    // goes over the lane's own vectors whose best reaches the bound and `least`; uniform over the wave
+    // goes over the vectors of the lanes whose best reaches the bound -- a handful, so the wave shares them out, a vector per
+    // lane -- and hands on what reaches `least` as well; uniform over the wave
+    const unsigned long long who = __ballot(in);
+    const int n_in = __popcll(who), ahead = (int)__builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0u));
+    const int ids = __builtin_amdgcn_ds_permute(4 * (in ? ahead : n_in + lane - ahead), lane);      // lane j: the j-th of them
+    const int wave0 = tid - lane, each = rp.body > wave0 ? (rp.body - wave0 + NT - 1) / NT : 0, pairs = n_in * each;
     auto look = [&](auto&& least, auto&& take) __attribute__((always_inline)) {
-      if (!__ballot(in)) return;
-      for (int v = tid; v - tid + (tid & ~63) < rp.body; v += NT) {
+      for (int p0 = 0; p0 < pairs; p0 += 64) {
+        const int p = p0 + lane < pairs ? p0 + lane : pairs - 1, j = p / each;
+        const int v = wave0 + __builtin_amdgcn_ds_bpermute(4 * j, ids) + (p - j * each) * NT;
+        const bool have = p0 + lane < pairs && v < rp.body;
         Vec<DT> q;
-        const bool have = in && v < rp.body;
         if (have) q.q = body[v];
         float vm = NEG_INF;
         bool nan = false;
@@ -464,12 +516,8 @@ __global__ __launch_bounds__(64) void symbol_rows_join_kernel(Logits l, const in
   float log_s, h;
   finish(st, &log_s, &h);
   if (top > 0) {
-    // four parts' first places a group: the same bound as over a row's lanes
-    unsigned k = key[0], o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0xB1, 0xF, 0xF, true);
-    k = k > o ? k : o;
-    o = (unsigned)__builtin_amdgcn_mov_dpp((int)k, 0x4E, 0xF, 0xF, true);
-    k = k > o ? k : o;
-    const unsigned bound = nth_of_16((unsigned)__shfl((int)k, 4 * (lane & 15), 64), top, lane);
+    // four (two) parts' first places a group: the same bound as over a row's lanes
+    const unsigned bound = group_bound(max_with<0xB1>(key[0]), top, lane);
     __threadfence_block();
 #pragma unroll
     for (int j = 0; j < DVC_MAX_TOP; ++j)
