@@ -162,7 +162,7 @@ extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t
   a.segments = p.segments;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool aligned = in_w % 4 == 0 && p.wo % 4 == 0 && reinterpret_cast<uintptr_t>(grad_out) % 16 == 0 &&
-                       4LL * out_channels * p.ho * p.wo < (1LL << 31);
+                       16LL * p.ho * p.wo < (1LL << 31);
   if (int rc = aligned ? launch_aligned(ksize, stride, a, p, st) : launch_any(ksize, stride, a, p, st)) return rc;
   const long long units = (long long)out_channels * p.taps * ((cin + 3) / 4) + (out_channels + 3) / 4;
   // Blocks of 64 units by 16 groups (64->64 3x3 in 256 slabs: 8 us, 16 by 64 10); where those are fewer than half the CUs, 16 by

@@ -192,24 +192,29 @@ struct Stager {
   const unsigned flip;
   int per_n, xlive;             // tiles per sample, this wave's channels that exist
   bool together;                // this wave's channels all exist and lie in one source: adjacent planes
-  unsigned plane_bytes, gplane, gsample;
+  unsigned plane_bytes, gplane;
   Plane xp[XPW];
-  // gradient units: unit u = stid + 64 NS i is unit u % GE of channel u / GE
-  unsigned gsrc[GLOADS];        // this lane's channel; past the last: none
-  int gdst[GLOADS];
-  float gsum[GLOADS];
+  // Gradients.  AL: 16-byte units, unit u = stid + 64 NS i is unit u % GE of channel u / GE: a load is CPL whole channels.  Else
+  // dwords, so that a load reads whole row pieces wherever they start (16-byte units in four dwords each met four times the
+  // cache lines: 64->64 3x3 at 32x255x253 540 us, now 471): a load is 64 pixels of one of this wave's GPW channels, LPC loads a channel.  Either way what
+  // differs from load to load is uniform, in the descriptor, and the lanes' offsets are found once a tile.
+  static constexpr int CPL = 64 / G::GE, GPW = G::GCH / G::NS, LPC = AL ? 1 : G::TH * TW / 64;
+  static constexpr int GREGS = AL ? GLOADS : GPW * LPC, GSUMS = AL ? GLOADS : GPW;
+  static_assert(AL || (G::TH * TW % 64 == 0 && 64 % TW == 0), "a channel's pixels are whole loads of whole rows");
+  typedef typename std::conditional<AL, float4, float>::type GReg;
+  int co0;
+  float gsum[GSUMS];
   unsigned xk[XPW][XSLOTS], xs[XPW][XSLOTS], xs2[AL ? 1 : XPW][AL ? 1 : XSLOTS];
   int mask[XSLOTS];             // codes of a dword inside the row (not AL; none: it lies outside the plane)
   int cut[XSLOTS];              // codes of a dword before a block's end (not AL)
   unsigned shift[XSLOTS];       // bits by which a dword was read early (not AL)
-  float4 gr[GLOADS];
+  GReg gr[GREGS];
 
-  __device__ __forceinline__ Stager(const Args& args, int lane_, int sw_, int co0, int ci0, unsigned flip_)
-      : a(args), lane(lane_), sw(sw_), stid(64 * sw_ + lane_), flip(flip_) {
+  __device__ __forceinline__ Stager(const Args& args, int lane_, int sw_, int co0_, int ci0, unsigned flip_)
+      : a(args), lane(lane_), sw(sw_), stid(64 * sw_ + lane_), flip(flip_), co0(co0_) {
     per_n = a.tiles_x * a.tiles_y;
     plane_bytes = 32u * (unsigned)a.blocks;
     gplane = (unsigned)(a.ho * a.wo);
-    gsample = 4u * (unsigned)a.cout * gplane;      // AL: below 2^31 (checked on the host)
     xlive = a.cin - (ci0 + XPW * sw);
     // (finding a channel's plane is some 80 scalar instructions: 16 times that was a fifth of a one-tile workgroup's time)
     const int c0 = ci0 + XPW * sw, c1 = c0 + XPW;
@@ -225,12 +230,7 @@ struct Stager {
       for (int c = 1; c < XPW; ++c) xp[c] = xp[0];
     }
 #pragma unroll
-    for (int i = 0; i < GLOADS; ++i) {
-      const int u = stid + 64 * G::NS * i, ch = u / G::GE, e = u - ch * G::GE;
-      gsrc[i] = co0 + ch < a.cout ? (unsigned)(co0 + ch) : 0xffffffffu;
-      gdst[i] = G::XBYTES + (ch * G::GUNITS + e) * 16;
-      gsum[i] = 0.f;
-    }
+    for (int i = 0; i < GSUMS; ++i) gsum[i] = 0.f;
   }
 
   // request tile t (past the last: zeros)
@@ -292,26 +292,32 @@ struct Stager {
         }
       }
     }
-    // gradients: four adjacent pixels of a row
+    if constexpr (AL) {
+      // four adjacent pixels of a row
+      const int e = lane % G::GE, oy = oy0 + 4 * e / TW, ox = ox0 + 4 * e % TW;
+      const unsigned at = oy < a.ho && ox < a.wo ? 4u * ((unsigned)(lane / G::GE) * gplane + (unsigned)(oy * a.wo + ox)) : 0x80000000u;
 #pragma unroll
-    for (int i = 0; i < GLOADS; ++i) {
-      const int e = stid % G::GE;
-      const int oy = oy0 + 4 * e / TW, ox = ox0 + 4 * e % TW;
-      const bool ok = gsrc[i] != 0xffffffffu && oy < a.ho && ox < a.wo;
-      if constexpr (AL) {
-        const unsigned at = ok ? 4u * (gsrc[i] * gplane + (unsigned)(oy * a.wo + ox)) : 0x80000000u;
+      for (int i = 0; i < GLOADS; ++i) {
+        const int ch = co0 + (sw + G::NS * i) * CPL, live = there ? (a.cout - ch < CPL ? a.cout - ch : CPL) : 0;
         gr[i] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(
-            rsrc((unsigned long long)a.g + (unsigned long long)(unsigned)n * gsample, there ? gsample : 0u), at, 0, 0));
-      } else {
-        // (one unaligned 16-byte load per unit, masked when it is stored, was slower: 64->64 3x3 at 32x255x253 638 against 545 us)
-        const float* const p = a.g + ((unsigned long long)(unsigned)n * a.cout + (ok ? gsrc[i] : 0u)) * gplane + (ok ? oy * a.wo + ox : 0);
-        gr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (ok && there) {
-          gr[i].x = p[0];
-          if (ox + 1 < a.wo) gr[i].y = p[1];
-          if (ox + 2 < a.wo) gr[i].z = p[2];
-          if (ox + 3 < a.wo) gr[i].w = p[3];
-        }
+            rsrc((unsigned long long)a.g + 4ull * ((unsigned long long)(unsigned)n * a.cout + (live > 0 ? ch : 0)) * gplane,
+                 live > 0 ? 4u * (unsigned)live * gplane : 0u), at, 0, 0));      // (CPL planes below 2^31 bytes: checked on the host)
+      }
+    } else {
+      unsigned at[LPC];
+#pragma unroll
+      for (int p = 0; p < LPC; ++p) {
+        const int oy = oy0 + (64 * p + lane) / TW, ox = ox0 + lane % TW;
+        at[p] = oy < a.ho && ox < a.wo ? 4u * (unsigned)(oy * a.wo + ox) : 0x80000000u;
+      }
+#pragma unroll
+      for (int c = 0; c < GPW; ++c) {
+        const int ch = co0 + GPW * sw + c;
+        const bool live = there && ch < a.cout;
+        const __amdgpu_buffer_rsrc_t rg = rsrc((unsigned long long)a.g + 4ull * ((unsigned long long)(unsigned)n * a.cout + (live ? ch : 0)) * gplane,
+                                               live ? 4u * gplane : 0u);
+#pragma unroll
+        for (int p = 0; p < LPC; ++p) gr[c * LPC + p] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rg, at[p], 0, 0));
       }
     }
   }
@@ -352,10 +358,23 @@ struct Stager {
         }
       }
     }
+    if constexpr (AL) {
+      char* const to = buf + G::XBYTES + (sw * CPL + lane / G::GE) * G::GUNITS * 16 + lane % G::GE * 16;
 #pragma unroll
-    for (int i = 0; i < GLOADS; ++i) {
-      *reinterpret_cast<float4*>(buf + gdst[i]) = gr[i];
-      gsum[i] += (gr[i].x + gr[i].y) + (gr[i].z + gr[i].w);
+      for (int i = 0; i < GLOADS; ++i) {
+        *reinterpret_cast<float4*>(to + i * G::NS * CPL * G::GUNITS * 16) = gr[i];
+        gsum[i] += (gr[i].x + gr[i].y) + (gr[i].z + gr[i].w);
+      }
+    } else {
+      char* const to = buf + G::XBYTES + GPW * sw * G::GUNITS * 16 + 4 * lane;
+#pragma unroll
+      for (int c = 0; c < GPW; ++c) {
+#pragma unroll
+        for (int p = 0; p < LPC; ++p) {
+          *reinterpret_cast<float*>(to + c * G::GUNITS * 16 + 256 * p) = gr[c * LPC + p];
+          gsum[c] += gr[c * LPC + p];
+        }
+      }
     }
   }
 
@@ -364,14 +383,15 @@ struct Stager {
     else store_as<false>(buf);
   }
 
-  // the bias gradient of what was staged: a channel's units are GE adjacent lanes
+  // the bias gradient of what was staged: a channel's sums are those of GE adjacent lanes (not AL: of all)
   __device__ __forceinline__ void bias(float* out) {
+    constexpr int LANES = AL ? G::GE : 64;
 #pragma unroll
-    for (int i = 0; i < GLOADS; ++i) {
+    for (int i = 0; i < GSUMS; ++i) {
       float v = gsum[i];
 #pragma unroll
-      for (int m = G::GE / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-      if (stid % G::GE == 0) out[(stid + 64 * G::NS * i) / G::GE] = v;
+      for (int m = LANES / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+      if (lane % LANES == 0) out[AL ? (stid + 64 * G::NS * i) / G::GE : GPW * sw + i] = v;
     }
   }
 };
@@ -400,16 +420,19 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
   if (KS != 7 && wave >= G::NM) {
     // ------------------------------------------------------------ staging
     Stager<G, AL> st(a, lane, wave - G::NM, co0, ci0, flip);
-    int buf = 0;
-    st.load(part);
-    st.store(lds);
-    st.load(part + nsplit);
-    __syncthreads();
-    for (int t = part; t < a.n_tiles; t += nsplit) {
-      st.store(lds + (G::BUF - buf));        // tile t + nsplit (zeros past the last)
-      st.load(t + 2 * nsplit);
-      __syncthreads();
-      buf = G::BUF - buf;
+    // (one copy of the code from the first load on: a one-tile workgroup spends much of its time fetching instructions, 64->64
+    // stride 2 33 -> 26 us)
+    int buf = G::BUF;
+#pragma unroll 1
+    for (int t = part - 2 * nsplit; t < a.n_tiles; t += nsplit) {
+      const bool begun = t > part - 2 * nsplit;
+      if (begun && t + nsplit < a.n_tiles) st.store(lds + (G::BUF - buf));      // tile t + nsplit
+      // AL: past the last tile the descriptors are empty, and a branch here would have the loads waited for at its end
+      if (AL || t + 2 * nsplit < a.n_tiles) st.load(t + 2 * nsplit);
+      if (begun) {
+        __syncthreads();
+        buf = G::BUF - buf;
+      }
     }
     if (a.bias_partial != nullptr && cib == 0) st.bias(a.bias_partial + (long long)part * a.cout_pad + co0);
     return;
