@@ -497,6 +497,30 @@ def test_residual_block_on_the_tape(kw, fmt):
         assert torch.equal(a, c)
 
 
+@pytest.mark.parametrize("in_slope,out_slope", [(None, None), (0.1, None), (None, 0.01), (0.0, 0.2)])
+@pytest.mark.parametrize("which", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (1, 1, 0), (0, 1, 1)])
+def test_partly_frozen_convolution_on_the_tape(which, in_slope, out_slope):
+    """Only some of input, weight and bias have gradients: those are the ones of the whole, and the tape keeps codes only where
+    one of them reads them."""
+    from deepvideocodec_amd import autograd as A
+    gen = torch.Generator().manual_seed(9)
+    x, wt, b = torch.randn(2, 20, 9, 12, generator=gen).cuda(), torch.randn(24, 20, 3, 3, generator=gen).cuda(), torch.randn(24, generator=gen).cuda()
+    R = torch.randn(2, 24, 9, 12, generator=gen).cuda()
+    leaves = [t.clone().requires_grad_() for t in (x, wt, b)]
+    whole = torch.autograd.grad(A.conv2d(*leaves, in_slope=in_slope, out_slope=out_slope, storage="int8"), leaves, R)
+    some = [t.clone().requires_grad_(bool(w)) for t, w in zip((x, wt, b), which)]
+    y = A.conv2d(*some, in_slope=in_slope, out_slope=out_slope, storage="int8")
+    codes = any(t is not None and t.dtype == torch.uint8 for t in y.grad_fn.saved_tensors)
+    assert codes == bool(which[1] or (which[0] and in_slope is not None))
+    got = torch.autograd.grad(y, [t for t in some if t.requires_grad], R)
+    want = [t for t, w in zip(whole, which) if w]
+    for a, c, t in zip(got, want, [t for t in some if t.requires_grad]):
+        if t is some[2]:       # a bias alone is summed by another kernel
+            assert float((a - c).abs().max()) <= 2 * 9 * 12 * 2.0 ** -24 * float(R.abs().sum((0, 2, 3)).max())
+        else:
+            assert torch.equal(a, c)
+
+
 def test_squeeze_excite_pieces_on_the_tape():
     from deepvideocodec_amd import autograd as A, ops
     torch.manual_seed(0)
