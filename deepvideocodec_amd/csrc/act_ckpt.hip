@@ -102,10 +102,12 @@ __device__ __forceinline__ unsigned encode4(float4 v, unsigned amax, unsigned* s
   const bool poison = amax >= 0x7f800000u;
   const float inv = poison ? 0.f : __uint_as_float((unsigned)(254 - s) << 23);
   *scale = poison ? 255u : (unsigned)s;
-  // the largest magnitude whose code does not restore to 2^128: it matters in the topmost binade only
-  constexpr float kMost = FMT == DVC_CKPT_INT8 ? 0x1.f8p127f : 0x1.ep127f;
-  const float a0 = fminf(fabsf(v.x), kMost) * inv, a1 = fminf(fabsf(v.y), kMost) * inv;
-  const float a2 = fminf(fabsf(v.z), kMost) * inv, a3 = fminf(fabsf(v.w), kMost) * inv;
+  // the largest magnitude whose code does not restore to 2^128.  e4m3: 240 steps of the largest scale; in the next one down
+  // nothing is that large.  int8: 63 steps of the largest scale, while all 127 of the next one down restore below 2^128.
+  // (Everywhere else a bound that only infinities and NaN, whose codes are zeros, meet.)
+  const float most = FMT != DVC_CKPT_INT8 ? 0x1.ep127f : s == 249 ? 0x1.f8p127f : 0x1.fffffep127f;
+  const float a0 = fminf(fabsf(v.x), most) * inv, a1 = fminf(fabsf(v.y), most) * inv;
+  const float a2 = fminf(fabsf(v.z), most) * inv, a3 = fminf(fabsf(v.w), most) * inv;
   unsigned mag;
   if (FMT == DVC_CKPT_INT8) {
     // adding 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits
