@@ -257,6 +257,69 @@ def test_alternatives_in_planes_of_very_many_classes(dtype, classes):
         same(r.top_log_prob, tl, tol)
 
 
+def sums64(x):
+    """float64, classes first: log p of all, entropies."""
+    lp = x.double() - x.double().logsumexp(0, keepdim=True)
+    return lp, -torch.where(lp == NEG, 0.0, lp.exp() * lp).sum(0)
+
+
+@pytest.mark.parametrize("values", ["whole", "normal"])
+@pytest.mark.parametrize("n,classes,top", [(2048, 131072, 0), (2048, 65536, 2), (64, 131072, 8), (1, 131072, 16), (1, 100003, 0)])
+def test_sums_over_very_many_classes_in_planes(n, classes, top, values):
+    """Sums over a hundred thousand classes keep fp32's accuracy whatever a lane has to add up (n samples of the same 8 x 8
+    pixels: from 2048 on a lane takes every class): a lane adds at most 263 terms in fp32 in a row, its share is one of at
+    most 16.  Whole logits: the terms repeat, so that the roundings of a long fp32 sum do not cancel."""
+    from deepvideocodec_amd import ops
+    g = torch.Generator().manual_seed(31 + classes)
+    place = (1, classes, 8, 8)
+    x = (torch.randint(-3, 4, place, generator=g) if values == "whole" else 3 * torch.randn(place, generator=g)).bfloat16().cuda()
+    sym = torch.randint(0, classes, (1, 1, 8, 8), generator=g, dtype=torch.int32).cuda()
+    lp, ent = sums64(x.view(classes, 64))
+    given = lp.gather(0, sym.view(1, 64).long())
+    r = ops.symbol_log_probs(x.expand(n, *place[1:]), sym.expand(n, 1, 8, 8).contiguous(), top)
+    tol = (2 * float(lp.abs().max()) + 16 + 263 + 16) * 2.0 ** -23
+    assert float((r.log_prob.view(n, 64) - given).abs().max()) <= tol
+    assert bool(((r.entropy.view(n, 64) - ent).abs() <= tol * (2 + ent)).all())
+    if top:
+        best = torch.sort(x.view(classes, 64).float(), dim=0, descending=True, stable=True).indices[:top]
+        assert torch.equal(r.top_symbol.view(n, top, 64), best.to(torch.int32).expand(n, top, 64))
+        assert float((r.top_log_prob.view(n, top, 64) - lp.gather(0, best)).abs().max()) <= tol
+
+
+def test_transposed_rows_of_very_many_classes():
+    """(N, classes) logits whose classes lie apart: values and gradient, with a masked row, a NaN and an infinity."""
+    from deepvideocodec_amd import ops
+    v, n = 1 << 20, 64
+    g = torch.Generator().manual_seed(32)
+    xt = torch.randint(-3, 4, (v, n), generator=g).bfloat16()
+    xt[:, 5] = NEG
+    xt[77777, 6] = float("nan")
+    xt[7, 7] = float("inf")
+    xt[:, 8] = torch.where(torch.arange(v) == 900001, 2.0, NEG)
+    xt[:, 9] = torch.arange(v) * (1.0 / 4096)                  # a maximum that keeps growing
+    xt = xt.cuda()
+    sym = torch.randint(0, v, (n,), generator=g, dtype=torch.int32).cuda()
+    fine = [i for i in range(n) if i not in (5, 6, 7)]
+    lp, ent = sums64(xt[:, fine])
+    spread = float(lp[torch.isfinite(lp)].abs().max().clamp(max=104))
+    # 263 terms in a row, 16 shares; the growing maximum rescales each of its 1024 stretches, a rounding each
+    tol = (2 * spread + 16 + 263 + 16 + 1024) * 2.0 ** -23
+    gl = torch.randn(n, generator=g).cuda()
+    for top in (0, 8):
+        r = ops.symbol_log_probs(xt.t(), sym, top)
+        assert r.log_prob[5] == NEG and r.entropy[5] == 0 and bool(r.log_prob[6:8].isnan().all()) and bool(r.entropy[6:8].isnan().all())
+        given = lp.gather(0, sym[fine].view(1, -1).long())[0]
+        at = torch.isfinite(given)
+        assert torch.equal(r.log_prob[fine][~at].double(), given[~at])
+        assert bool(((r.log_prob[fine] - given)[at].abs() <= tol + given[at].abs() * 2.0 ** -23).all())
+        assert bool(((r.entropy[fine] - ent).abs() <= tol * (2 + ent)).all())
+        got = ops.symbol_log_probs_backward(xt.t(), sym, r.stats, r.entropy, gl, gl).t()[:, fine].double()
+        p, a = lp.exp(), gl[fine].double()
+        want = -p * a * (1 + torch.where(p == 0, 0.0, lp + ent)) + a * (torch.arange(v, device="cuda")[:, None] == sym[fine])
+        bound = tol * a.abs() * (3 + 2 * ent) + want.abs() * 2.0 ** -8 + torch.finfo(torch.bfloat16).smallest_normal
+        assert bool(((got - want).abs() <= bound).all())
+
+
 def test_one_row_for_all_sites():
     """Expanded logits (no stride between rows), also where rows share waves."""
     from deepvideocodec_amd import ops
