@@ -355,11 +355,15 @@ __global__ __launch_bounds__(256) void symbol_rows_kernel(Logits l, const int* s
   const float end_x = has_end ? Elem<DT>::up(row[end_v]) : NEG_INF;
   if (has_end) st.add(end_x);
   constexpr int U = 4;                  // vectors in flight per lane
+  constexpr int STRETCH = kChain / N * NT;      // vectors over which a lane adds up kChain classes
+  WideStat wide;
+  wide.clear();
   for (int j = tid; j < rp.body; j += U * NT) {
     Vec<DT> q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (j + u * NT < rp.body) q[u].q = body[j + u * NT];
+    if (WAVES > 1 && j >= STRETCH && (j - tid) % STRETCH == 0) wide.take(&st);      // (a row of one wave is shorter)
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (j + u * NT < rp.body) {
@@ -369,6 +373,7 @@ __global__ __launch_bounds__(256) void symbol_rows_kernel(Logits l, const int* s
         add_many<N>(&st, x);
       }
   }
+  if (WAVES > 1 && rp.body > STRETCH) wide.give(&st);
 
   // what the lane's best class is worth; a lane that met a NaN or +inf looks again (its maximum ignores NaN)
   unsigned best = 0;

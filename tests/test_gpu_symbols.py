@@ -286,6 +286,32 @@ def test_sums_over_very_many_classes_in_planes(n, classes, top, values):
         assert float((r.top_log_prob.view(n, top, 64) - lp.gather(0, best)).abs().max()) <= tol
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,classes,top", [(512, (1 << 24) + 5, 0), (512, 1000003, 8), (1, (1 << 24) + 5, 8), (3, 300007, 1)])
+def test_sums_over_very_long_rows(n, classes, top, dtype):
+    """The same for rows (n sites over one row): with 512 of them a workgroup takes a whole row, 65536 classes a lane.  A lane adds
+    at most 256 + 2 terms in a row, then come 64 lanes and at most 64 parts."""
+    from deepvideocodec_amd import ops
+    g = torch.Generator().manual_seed(33)
+    x = torch.randint(-3, 4, (classes,), generator=g).to(dtype).cuda()
+    sym = torch.randint(0, classes, (n,), generator=g, dtype=torch.int32).cuda()
+    lp, ent = sums64(x.view(classes, 1))
+    r = ops.symbol_log_probs(x.expand(n, classes), sym, top)
+    tol = (2 * float(lp.abs().max()) + 16 + 258 + 16) * 2.0 ** -23
+    assert float((r.log_prob - lp[sym.long(), 0]).abs().max()) <= tol
+    assert float((r.entropy - ent).abs().max()) <= tol * (2 + float(ent))
+    if top:
+        best = torch.nonzero(x == 3)[:top, 0]
+        assert torch.equal(r.top_symbol, best.to(torch.int32).expand(n, top))
+        assert float((r.top_log_prob - lp[best, 0]).abs().max()) <= tol
+    for bad in (float("nan"), float("inf")):
+        x[classes - 3] = bad
+        r = ops.symbol_log_probs(x.expand(n, classes), sym, top)
+        assert bool(r.log_prob.isnan().all()) and bool(r.entropy.isnan().all())
+        if top:
+            assert bool((r.top_symbol[:, 0] == classes - 3).all()) and torch.equal(r.top_symbol[:, 1:], best[:top - 1].to(torch.int32).expand(n, top - 1))
+
+
 def test_transposed_rows_of_very_many_classes():
     """(N, classes) logits whose classes lie apart: values and gradient, with a masked row, a NaN and an infinity."""
     from deepvideocodec_amd import ops
