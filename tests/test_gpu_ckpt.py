@@ -310,6 +310,56 @@ def test_weight_gradient_of_long_sums(k, stride, cin, cout, h, w, batch):
     assert torch.equal(gb.double(), rows.sum(1))
 
 
+def wgrad64_gpu(x, g, k, stride):
+    """The same of fp32 GPU tensors, in float64, sample by sample."""
+    n, cout, ho, wo = g.shape
+    cin, p = x.size(1), k // 2
+    gw = torch.zeros(cout, cin, k, k, dtype=torch.float64, device=x.device)
+    for i in range(n):
+        xp = F.pad(x[i], (p, p, p, p)).double()
+        rows = g[i].double().reshape(cout, -1)
+        for ky in range(k):
+            for kx in range(k):
+                cols = xp[:, ky:ky + (ho - 1) * stride + 1:stride, kx:kx + (wo - 1) * stride + 1:stride].reshape(cin, -1)
+                gw[:, :, ky, kx] += rows @ cols.t().contiguous()
+    return gw
+
+
+def real_sums(k, stride, cin, cout, h, w, batch, fmt):
+    """-> error of a weight gradient of random real numbers, in units of the gradient's root mean square."""
+    from deepvideocodec_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(34)
+    ho, wo = (h + 2 * (k // 2) - k) // stride + 1, (w + 2 * (k // 2) - k) // stride + 1
+    ck = ops.act_checkpoint(torch.empty(batch, cin, h, w, device="cuda").normal_(generator=gen), fmt=fmt)
+    g = torch.empty(batch, cout, ho, wo, device="cuda").normal_(generator=gen)
+    want = wgrad64_gpu(ops.act_restore(ck), g, k, stride)
+    return (ops.conv2d_wgrad_ckpt(ck, g, (cout, cin, k, k), stride).double() - want) / want.square().mean().sqrt()
+
+
+@pytest.mark.parametrize("k,stride,cin,cout,h,w,batch,fmt", [
+    (3, 1, 64, 64, 256, 256, 16, "int8"), (3, 1, 64, 64, 256, 256, 32, "e4m3"),      # one slab in time, two
+    (3, 1, 64, 64, 255, 253, 8, "int8"), (3, 1, 96, 33, 128, 128, 8, "e4m3"), (3, 1, 32, 32, 256, 256, 16, "int8"),
+    (3, 1, 40, 24, 255, 129, 8, "e4m3"), (3, 1, 3, 64, 256, 256, 16, "int8"), (3, 1, 64, 3, 256, 256, 8, "int8"),
+    (3, 1, 128, 128, 16, 16, 64, "e4m3"), (3, 2, 64, 64, 256, 256, 8, "int8"), (3, 2, 32, 64, 255, 257, 8, "e4m3"),
+    (1, 1, 64, 64, 256, 256, 32, "int8"), (1, 1, 32, 48, 255, 255, 8, "e4m3"), (1, 2, 64, 64, 256, 256, 8, "int8"),
+    (7, 1, 32, 64, 128, 128, 32, "e4m3"), (7, 1, 16, 2, 255, 253, 4, "int8"), (1, 1, 1024, 1024, 96, 128, 1, "int8")])
+def test_weight_gradient_of_long_sums_of_real_numbers(k, stride, cin, cout, h, w, batch, fmt):
+    """All three parts of the gradient arrive in every form and at every place of a tile.  A slab is at most 512 row pieces of
+    three matrix instructions that round twice: 3072 roundings of a sum that grows like a random walk, 2^-24 / sqrt(3) of
+    its size each, come to sqrt(3072 / 2) 2^-24 / sqrt(3) = 1.4e-6 of the result.  Without the third part every gradient is
+    cut off by 2^-17 (5.5e-6 on average, all towards zero); without the second by 2^-9."""
+    assert float(real_sums(k, stride, cin, cout, h, w, batch, fmt).square().mean().sqrt()) <= 3e-6
+
+
+@pytest.mark.parametrize("k,stride,cin,cout,h,w,batch", [(3, 1, 64, 64, 256, 256, 32), (1, 1, 1024, 1024, 128, 128, 4), (1, 1, 1024, 512, 128, 128, 4),
+                                                         (7, 1, 512, 512, 64, 256, 2)])
+def test_weight_gradient_does_not_drift(k, stride, cin, cout, h, w, batch):
+    """The matrix instruction's cuts are all downwards; over an even number of slabs -- over workgroups (the first: 256 of them, two
+    slabs each) or in time (one workgroup per block, 16 slabs) -- they cancel.  Without the alternating signs the mean error is
+    2e-6 and 2.3e-7 of the results' size; what chance leaves of it is 7e-7 / sqrt(results), 4e-9 or less."""
+    assert abs(float(real_sums(k, stride, cin, cout, h, w, batch, "int8").mean())) <= 2e-8
+
+
 @pytest.mark.parametrize("e", [-60, -100, -118, 60, 100])
 def test_weight_gradient_of_very_small_and_large_gradients(e):
     """A power of two on the gradient is one on the result, as long as nothing leaves the normal numbers."""
