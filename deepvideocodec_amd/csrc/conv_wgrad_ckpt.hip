@@ -8,7 +8,8 @@ int launch_aligned(int ks, int stride, const Args& a, const Plan& p, hipStream_t
 
 namespace {
 
-// gW[co][ci][tap] = sum over slabs of partial[slab][tap][co][ci], gB[co] likewise over splits (units past the weight's).  A lane
+// gW[co][ci][tap] = sum over slabs of partial[slab][tap][co][ci], gB[co] likewise over splits (units past the weight's); `more`: added
+// to what they hold.  A lane
 // takes four adjacent input channels (rows of a slab are padded to 32), a block UNITS such units; each of its GROUPS groups of
 // lanes adds every GROUPS-th slab, with the loads of four slabs in flight, and the sums are added in a fixed order.
 __device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
@@ -16,7 +17,7 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(
 template <int UNITS, int GROUPS>
 __global__ __launch_bounds__(UNITS * GROUPS) void wgrad_ckpt_reduce_kernel(const float* partial, float* gw, int slabs, int nsplit, int taps,
                                                                        int cout, int cin, int cout_pad, int cin_pad,
-                                                                       const float* bias_partial, float* gb) {
+                                                                       const float* bias_partial, float* gb, int more) {
   __shared__ float4 part[GROUPS][UNITS];
   const unsigned cin4 = (unsigned)(cin + 3) / 4, units = (unsigned)cout * (unsigned)taps * cin4;
   const unsigned all = units + (gb != nullptr ? (unsigned)(cout + 3) / 4 : 0u);
@@ -46,16 +47,19 @@ __global__ __launch_bounds__(UNITS * GROUPS) void wgrad_ckpt_reduce_kernel(const
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (weight) {
-          if ((int)ci + j < cin) gw[((long long)co * cin + ci + j) * taps + tap] = r[j];
+          float* const to = gw + ((long long)co * cin + ci + j) * taps + tap;
+          if ((int)ci + j < cin) *to = more ? *to + r[j] : r[j];
         } else {
           const int c = (int)(4 * (i - units)) + j;
-          if (c < cout) gb[c] = r[j];
+          if (c < cout) gb[c] = more ? gb[c] + r[j] : r[j];
         }
       }
     }
     __syncthreads();
   }
 }
+
+constexpr long long kSlabBytes = 128ll << 20;
 
 int make_plan(int cout, int cin, int ks, int stride, int batch, int h, int w, Plan* p, const char* who) {
   DVC_REQUIRE(ks == 1 || ks == 3 || ks == 7, "%s: ksize=%d unsupported", who, ks);
@@ -88,13 +92,20 @@ int make_plan(int cout, int cin, int ks, int stride, int batch, int h, int w, Pl
   // A running sum is rounded twice per matrix instruction, so a slab ends after 256 row pieces of a wave (768 instructions;
   // 64->64 3x3 at 32x256x256, 512 pieces per wave: relative error 7e-7 in two slabs, 1.0e-6 in one); 7x7, whose slabs are
   // five times as large, after 512
-  const int kg = ks == 7 ? 1 : 4 / (p->mt * p->ct), pieces = p->th * p->tw / 16 / kg;
-  p->seg_tiles = (ks == 7 ? 512 : 256) / pieces;
+  p->kg = ks == 7 ? 1 : 4 / (p->mt * p->ct);
+  p->seg_tiles = (ks == 7 ? 512 : 256) / (p->th * p->tw / 16 / p->kg);
   const int most = (p->n_tiles + p->nsplit - 1) / p->nsplit;      // tiles of a workgroup
-  p->segments = (most + p->seg_tiles - 1) / p->seg_tiles;
-  p->slabs = p->segments * p->nsplit * kg;
+  p->all_segments = (most + p->seg_tiles - 1) / p->seg_tiles;
+  // Slabs in time do not add up in memory: beyond 128 MiB of them the tiles are dealt out over several launches, each with a
+  // reduction that adds to the result (192->192 3x3 at 32x256x256: 693 MB in one launch).  Adding to the slabs
+  // inside the kernel instead needs less, but is slower by the latency of reading them (64->64 3x3 at 32x256x256 460 -> 485 us,
+  // 192->192 at 4x256x256 647 -> 728).
+  const long long one = 4ll * p->nsplit * p->kg * p->taps * p->cout_pad * p->cin_pad, most_at_once = one < kSlabBytes ? kSlabBytes / one : 1;
+  const long long launches = (p->all_segments + most_at_once - 1) / most_at_once;
+  p->segments = (int)((p->all_segments + launches - 1) / launches);
   return DVC_OK;
 }
+inline long long slab_floats(const Plan& p) { return (long long)p.segments * p.nsplit * p.kg * p.taps * p.cout_pad * p.cin_pad; }
 
 int check_srcs(const DvcCkpt* srcs, int n_src, int* cin, const char* who) {
   DVC_REQUIRE(srcs != nullptr && n_src >= 1 && n_src <= DVC_MAX_SRC, "%s: n_src=%d not in 1..%d", who, n_src, DVC_MAX_SRC);
@@ -118,7 +129,7 @@ extern "C" int64_t dvc_conv2d_wgrad_ckpt_scratch_floats(int32_t cout, int32_t ci
                                                         int32_t batch, int32_t in_h, int32_t in_w) {
   Plan p;
   if (int rc = make_plan(cout, cin, ksize, stride, batch, in_h, in_w, &p, "dvc_conv2d_wgrad_ckpt_scratch_floats")) return rc;
-  return (int64_t)p.slabs * p.taps * p.cout_pad * p.cin_pad + (int64_t)p.nsplit * p.cout_pad;
+  return slab_floats(p) + (int64_t)p.nsplit * p.cout_pad;
 }
 
 extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t batch, int32_t in_h, int32_t in_w,
@@ -151,29 +162,35 @@ extern "C" int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t
   a.wo = p.wo;
   a.g = grad_out;
   a.partial = scratch;
-  a.bias_partial = grad_bias != nullptr ? scratch + (long long)p.slabs * p.taps * p.cout_pad * p.cin_pad : nullptr;
+  a.bias_partial = grad_bias != nullptr ? scratch + slab_floats(p) : nullptr;
   a.cout_pad = p.cout_pad;
   a.cin_pad = p.cin_pad;
   a.n_cib = p.n_cib;
   a.tiles_x = p.tiles_x;
   a.tiles_y = p.tiles_y;
-  a.n_tiles = p.n_tiles;
   a.seg_tiles = p.seg_tiles;
-  a.segments = p.segments;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool aligned = in_w % 4 == 0 && p.wo % 4 == 0 && reinterpret_cast<uintptr_t>(grad_out) % 16 == 0 &&
                        16LL * p.ho * p.wo < (1LL << 31);
-  if (int rc = aligned ? launch_aligned(ksize, stride, a, p, st) : launch_any(ksize, stride, a, p, st)) return rc;
   const long long units = (long long)out_channels * p.taps * ((cin + 3) / 4) + (out_channels + 3) / 4;
   // Blocks of 64 units by 16 groups (64->64 3x3 in 256 slabs: 8 us, 16 by 64 10); where those are fewer than half the CUs, 16 by
   // 64 (3->64 3x3 in 1024 slabs: 42 us in 10 blocks, 18 in 37); of few slabs 64 by 4.
 #define REDUCE(UNITS, GROUPS)                                                                                                        \
   hipLaunchKernelGGL((wgrad_ckpt_reduce_kernel<UNITS, GROUPS>), dim3((unsigned)((units + UNITS - 1) / UNITS < 16384 ? (units + UNITS - 1) / UNITS : 16384)), \
-                     dim3(UNITS * GROUPS), 0, st, scratch, grad_weight, p.slabs, p.nsplit, p.taps, out_channels, cin, p.cout_pad, p.cin_pad, \
-                     a.bias_partial, grad_bias)
-  if (p.slabs < 64) REDUCE(64, 4);
-  else if (units < 64 * 128) REDUCE(16, 64);
-  else REDUCE(64, 16);
+                     dim3(UNITS * GROUPS), 0, st, scratch, grad_weight, slabs, p.nsplit, p.taps, out_channels, cin, p.cout_pad, p.cin_pad, \
+                     a.bias_partial, grad_bias, a.seg0 != 0)
+  for (a.seg0 = 0; a.seg0 < p.all_segments; a.seg0 += p.segments) {
+    const long long step = (long long)p.nsplit * p.seg_tiles, end = step * (a.seg0 + p.segments);
+    a.segments = a.seg0 + p.segments < p.all_segments ? p.segments : p.all_segments - a.seg0;
+    a.tile0 = (int)(step * a.seg0);
+    a.n_tiles = end < p.n_tiles ? (int)end : p.n_tiles;
+    if (int rc = aligned ? launch_aligned(ksize, stride, a, p, st) : launch_any(ksize, stride, a, p, st)) return rc;
+    const int slabs = a.segments * p.nsplit * p.kg;
+    if (slabs < 64) REDUCE(64, 4);
+    else if (units < 64 * 128) REDUCE(16, 64);
+    else REDUCE(64, 16);
+    if (int rc = dvc::check_launch("wgrad_ckpt_reduce_kernel")) return rc;
+  }
 #undef REDUCE
-  return dvc::check_launch("wgrad_ckpt_reduce_kernel");
+  return DVC_OK;
 }

@@ -48,8 +48,10 @@ struct Args {
   float* partial;               // [slabs][taps][cout_pad][cin_pad], slab = (segment * splits + split) * KG + wave of the corner
   float* bias_partial;          // [splits][cout_pad], or null
   int cout_pad, cin_pad, n_cib;
-  int tiles_x, tiles_y, n_tiles;
+  int tiles_x, tiles_y;
+  int tile0, n_tiles;           // this launch's tiles: from tile0 up to n_tiles
   int seg_tiles, segments;      // tiles of a workgroup per slab, slabs of a workgroup and wave (segments * seg_tiles tiles or fewer)
+  int seg0;                     // slabs in time before this launch
 };
 
 __device__ __forceinline__ unsigned long long uniform64(unsigned long long v) {
@@ -422,7 +424,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
   // that drift cancels (64->64 3x3 at 32x256x256: relative error 2.0e-6 without, of which 93 % is drift; 1024->1024 1x1 at
   // 4x128x128, one workgroup per block and 16 slabs: mean error of the results 2.3e-7 of their size with all slabs alike).
   // An odd number leaves one slab's.  It costs nothing: the sign rides on the scale.
-  unsigned flip = ((unsigned)part & 1u) << 31;
+  unsigned flip = ((unsigned)(part + a.seg0) & 1u) << 31;
 
   if (KS != 7 && wave >= G::NM) {
     // ------------------------------------------------------------ staging
@@ -431,8 +433,8 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     // stride 2 33 -> 26 us)
     int buf = G::BUF;
 #pragma unroll 1
-    for (int t = part - 2 * nsplit; t < a.n_tiles; t += nsplit) {
-      const bool begun = t > part - 2 * nsplit;
+    for (int t = a.tile0 + part - 2 * nsplit; t < a.n_tiles; t += nsplit) {
+      const bool begun = t > a.tile0 + part - 2 * nsplit;
       if (begun && t + nsplit < a.n_tiles) st.store(lds + (G::BUF - buf));      // tile t + nsplit
       // AL: past the last tile the descriptors are empty, and a branch here would have the loads waited for at its end
       if (AL || t + 2 * nsplit < a.n_tiles) st.load(t + 2 * nsplit);
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
     else return 0;
   }();
   const bool late = wave >= 4;
-  int t = part, buf = 0;
+  int t = a.tile0 + part, buf = 0;
   if constexpr (KS == 7) {
     st.load(t);
     st.store(lds);
@@ -570,7 +572,7 @@ __global__ __launch_bounds__(512) void wgrad_ckpt_kernel(const Args a) {
 
 struct Plan {
   int ho, wo, tw, th, tiles_x, tiles_y, n_tiles, cout_pad, cin_pad, n_cib, blocks, nsplit, taps, mt, ct;
-  int seg_tiles, segments, slabs;      // tiles of a workgroup per slab, slabs in time, slabs in all
+  int kg, seg_tiles, segments, all_segments;      // waves per corner, tiles of a workgroup per slab, slabs in time of a launch and in all
 };
 
 template <class K>

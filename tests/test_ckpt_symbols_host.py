@@ -76,6 +76,20 @@ def test_weight_gradient_refusals():
     assert lib.dvc_conv2d_wgrad_ckpt_scratch_floats(4, 3, 3, 1, 1, 8, 8) > 0
 
 
+@pytest.mark.parametrize("cout,cin,k,stride,n,h,w", [
+    (64, 64, 3, 1, 32, 256, 256), (192, 192, 3, 1, 32, 256, 256), (512, 512, 3, 1, 32, 128, 128), (1024, 1024, 1, 1, 8, 512, 512),
+    (64, 32, 7, 1, 32, 256, 256), (512, 512, 7, 1, 8, 256, 256), (40, 24, 3, 2, 64, 512, 512), (3, 64, 3, 1, 512, 256, 256), (2, 16, 7, 1, 4, 16, 16)])
+def test_weight_gradient_scratch_does_not_grow_with_the_pixels(cout, cin, k, stride, n, h, w):
+    """One block of every tap for each of about 256 workgroups (64 x 64, 7x7: 32 x 32; of weights that alone give more blocks than
+    that, one block each) or 128 MiB, whichever is more, and a row of bias sums for each workgroup."""
+    side = 32 if k == 7 else 64
+    blocks = -(-cout // side) * -(-cin // side)
+    most = max((256 + blocks) * side * side * k * k, 128 << 18) + (256 + blocks) * (cout + side)
+    lib = _lib.load()
+    for m in (n, 4 * n, 64 * n):
+        assert 0 < lib.dvc_conv2d_wgrad_ckpt_scratch_floats(cout, cin, k, stride, m, h, w) <= most
+
+
 def test_symbol_refusals():
     lib = _lib.load()
 

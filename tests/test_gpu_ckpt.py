@@ -325,6 +325,37 @@ def wgrad64_gpu(x, g, k, stride):
     return gw
 
 
+@pytest.mark.parametrize("k,cin,cout,h,w,batch", [
+    (3, 192, 192, 256, 256, 6),      # 3072 tiles over 29 workgroups a block: four slabs in time, two launches of two
+    (3, 192, 160, 256, 253, 7),      # five: of three and two
+    (7, 64, 64, 42, 4740, 5),        # 8195 tiles over 64 workgroups: three slabs, in the second launch three tiles
+    (7, 64, 64, 42, 4739, 5),
+])
+def test_weight_gradient_over_several_launches(k, cin, cout, h, w, batch):
+    """Where the slabs would need more than 128 MiB, several launches add to the result: whole numbers, exact; a fixed order;
+    also into memory that held something else, and in a replayed graph."""
+    from deepvideocodec_amd import _lib, ops
+    gen = torch.Generator(device="cuda").manual_seed(k + cin)
+    x = torch.randint(-1, 2, (batch, cin, h, w), generator=gen, device="cuda").float()
+    g = torch.randint(-1, 2, (batch, cout, h, w), generator=gen, device="cuda").float()
+    assert batch * h * w < 1 << 24 and 4 * _lib.load().dvc_conv2d_wgrad_ckpt_scratch_floats(cout, cin, k, 1, batch, h, w) < 129 << 20
+    ck = ops.act_checkpoint(x)
+    want = wgrad64_gpu(x, g, k, 1)
+    for _ in range(2):
+        gw, gb = ops.conv2d_wgrad_ckpt(ck, g, (cout, cin, k, k), with_bias=True)
+        assert torch.equal(gw.double(), want) and torch.equal(gb.double(), g.double().sum((0, 2, 3)))
+        del gw, gb                            # (the next call's results lie where these were)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gw, gb = ops.conv2d_wgrad_ckpt(ck, g, (cout, cin, k, k), with_bias=True)
+    for _ in range(3):
+        gw.fill_(float("nan"))
+        gb.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(gw.double(), want) and torch.equal(gb.double(), g.double().sum((0, 2, 3)))
+
+
 def real_sums(k, stride, cin, cout, h, w, batch, fmt):
     """-> error of a weight gradient of random real numbers, in units of the gradient's root mean square."""
     from deepvideocodec_amd import ops
@@ -342,7 +373,8 @@ def real_sums(k, stride, cin, cout, h, w, batch, fmt):
     (3, 1, 40, 24, 255, 129, 8, "e4m3"), (3, 1, 3, 64, 256, 256, 16, "int8"), (3, 1, 64, 3, 256, 256, 8, "int8"),
     (3, 1, 128, 128, 16, 16, 64, "e4m3"), (3, 2, 64, 64, 256, 256, 8, "int8"), (3, 2, 32, 64, 255, 257, 8, "e4m3"),
     (1, 1, 64, 64, 256, 256, 32, "int8"), (1, 1, 32, 48, 255, 255, 8, "e4m3"), (1, 2, 64, 64, 256, 256, 8, "int8"),
-    (7, 1, 32, 64, 128, 128, 32, "e4m3"), (7, 1, 16, 2, 255, 253, 4, "int8"), (1, 1, 1024, 1024, 96, 128, 1, "int8")])
+    (7, 1, 32, 64, 128, 128, 32, "e4m3"), (7, 1, 16, 2, 255, 253, 4, "int8"), (1, 1, 1024, 1024, 96, 128, 1, "int8"),
+    (3, 1, 192, 192, 256, 256, 8, "e4m3")])
 def test_weight_gradient_of_long_sums_of_real_numbers(k, stride, cin, cout, h, w, batch, fmt):
     """All three parts of the gradient arrive in every form and at every place of a tile.  A slab is at most 512 row pieces of
     three matrix instructions that round twice: 3072 roundings of a sum that grows like a random walk, 2^-24 / sqrt(3) of
