@@ -206,7 +206,7 @@ struct Stager {
   static_assert(AL || (G::TH * TW % 64 == 0 && 64 % TW == 0), "a channel's pixels are whole loads of whole rows");
   typedef typename std::conditional<AL, float4, float>::type GReg;
   int co0;
-  float gsum[GSUMS];
+  float gsum[GSUMS], gbefore[GSUMS];      // the bias gradient's sums since the last slab's end and until then
   unsigned xk[XPW][XSLOTS], xs[XPW][XSLOTS], xs2[AL ? 1 : XPW][AL ? 1 : XSLOTS];
   int mask[XSLOTS];             // codes of a dword inside the row (not AL; none: it lies outside the plane)
   int cut[XSLOTS];              // codes of a dword before a block's end (not AL)
@@ -233,7 +233,7 @@ struct Stager {
       for (int c = 1; c < XPW; ++c) xp[c] = xp[0];
     }
 #pragma unroll
-    for (int i = 0; i < GSUMS; ++i) gsum[i] = 0.f;
+    for (int i = 0; i < GSUMS; ++i) gsum[i] = gbefore[i] = 0.f;
   }
 
   // request tile t (past the last: zeros)
@@ -387,6 +387,14 @@ struct Stager {
     else store_as<false>(buf);
     --left;
     flip ^= left == 0 ? 0x80000000u : 0u;
+    // (one sum over all tiles of a workgroup: 1024 equal gradients per channel over 2048 tiles off by 3e-5)
+    if (left == 0) {
+#pragma unroll
+      for (int i = 0; i < GSUMS; ++i) {
+        gbefore[i] += gsum[i];
+        gsum[i] = 0.f;
+      }
+    }
     left = left == 0 ? a.seg_tiles : left;
   }
 
@@ -395,7 +403,7 @@ struct Stager {
     constexpr int LANES = AL ? G::GE : 64;
 #pragma unroll
     for (int i = 0; i < GSUMS; ++i) {
-      float v = gsum[i];
+      float v = gbefore[i] + gsum[i];
 #pragma unroll
       for (int m = LANES / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
       if (lane % LANES == 0) out[AL ? (stid + 64 * G::NS * i) / G::GE : GPW * sw + i] = v;

@@ -392,6 +392,22 @@ def test_weight_gradient_does_not_drift(k, stride, cin, cout, h, w, batch):
     assert abs(float(real_sums(k, stride, cin, cout, h, w, batch, "int8").mean())) <= 2e-8
 
 
+@pytest.mark.parametrize("k,cin,cout,h,w,batch,chain", [
+    (1, 1024, 1024, 512, 512, 1, 32 + 32 + 2), (1, 1024, 1024, 511, 511, 1, 64 + 32 + 2), (7, 256, 256, 512, 512, 1, 64 + 2 + 4),
+    (3, 64, 64, 256, 256, 32, 32 + 2 + 1), (3, 576, 576, 128, 128, 16, 32 + 2 + 8), (3, 20, 24, 255, 253, 64, 256 + 1 + 1)])
+def test_bias_gradient_of_long_sums(k, cin, cout, h, w, batch, chain):
+    """One gradient per channel throughout: the terms of a sum are equal, so that the roundings of a long sum do not cancel.  `chain`:
+    the terms that a lane adds up between two slabs' ends, the slabs in time of a launch, the launches; besides, a lane adds
+    four pixels (2), 64 lanes are joined (6), then at most 16 groups of 16 workgroups (4 + 4 + 16)."""
+    from deepvideocodec_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(35)
+    g = torch.rand(1, cout, 1, 1, device="cuda", generator=gen).expand(batch, cout, h, w).contiguous()
+    ck = ops.act_checkpoint(torch.zeros(batch, cin, h, w, device="cuda"))
+    gw, gb = ops.conv2d_wgrad_ckpt(ck, g, (cout, cin, k, k), with_bias=True)
+    want = g[0, :, 0, 0].double() * (batch * h * w)
+    assert bool(((gb - want).abs() <= (chain + 32) * 2.0 ** -24 * want).all()) and not bool(gw.any())
+
+
 @pytest.mark.parametrize("e", [-60, -100, -118, 60, 100])
 def test_weight_gradient_of_very_small_and_large_gradients(e):
     """A power of two on the gradient is one on the result, as long as nothing leaves the normal numbers."""
