@@ -48,7 +48,8 @@ class _Conv2d(torch.autograd.Function):
             # input activation's derivative), the output activation's derivative as one bit per value
             need = ctx.needs_input_grad
             ctx.kept, tensors = _keep(srcs, in_slope, storage, need[0] or in_slope is not None and any(need[13:]))
-            ctx.save_for_backward(weight, ops.act_signs(out) if out_slope is not None else None, *tensors)
+            signs = out_slope is not None and (need[0] or need[1] or any(need[13:]))
+            ctx.save_for_backward(weight, ops.act_signs(out) if signs else None, *tensors)
         return out
 
     @staticmethod

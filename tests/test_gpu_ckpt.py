@@ -639,6 +639,23 @@ def test_partly_frozen_convolution_on_the_tape(which, in_slope, out_slope):
             assert torch.equal(a, c)
 
 
+def test_frozen_convolution_stores_nothing(monkeypatch):
+    """Where no gradient is asked for (a frozen layer behind frozen layers, under grad mode) nothing is coded, signs included."""
+    from deepvideocodec_amd import autograd as A, ops
+    gen = torch.Generator().manual_seed(10)
+    x, wt, b = torch.randn(1, 8, 9, 12, generator=gen).cuda(), torch.randn(8, 8, 3, 3, generator=gen).cuda(), torch.randn(8, generator=gen).cuda()
+    want = A.conv2d(x, wt, b, in_slope=0.1, out_slope=0.2)
+    calls = []
+    for name in ("act_signs", "act_checkpoint"):
+        monkeypatch.setattr(ops, name, lambda *a, name=name, f=getattr(ops, name), **k: (calls.append(name), f(*a, **k))[1])
+    y = A.conv2d(x, wt, b, in_slope=0.1, out_slope=0.2, storage="int8")
+    assert torch.equal(y, want) and not y.requires_grad and calls == []
+    y = A.conv2d(x, wt, b.requires_grad_(), in_slope=0.1, out_slope=0.2, storage="int8")
+    assert torch.equal(y, want) and calls == ["act_signs"]
+    (gb,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    assert float((gb - torch.where(want > 0, 1.0, 0.2).sum((0, 2, 3))).abs().max()) <= 9 * 12 * 2.0 ** -24 * 9 * 12
+
+
 def test_squeeze_excite_pieces_on_the_tape():
     from deepvideocodec_amd import autograd as A, ops
     torch.manual_seed(0)
