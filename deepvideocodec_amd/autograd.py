@@ -109,8 +109,8 @@ def _keep(srcs, slope, fmt, values):
 
 
 def _kept(kept, tensors):
-    return [_ShapeOnly(shape) if fmt is None else ops.ActCheckpoint(tensors[2 * i], tensors[2 * i + 1], shape, fmt)
-            for i, (shape, fmt) in enumerate(kept)]
+    tensors = iter(tensors)
+    return [_ShapeOnly(shape) if fmt is None else ops.ActCheckpoint(next(tensors), next(tensors), shape, fmt) for shape, fmt in kept]
 
 
 # the adjoints that read a stored activation, whichever way it was stored
@@ -186,10 +186,12 @@ class _ResBlock(torch.autograd.Function):
             ctx.kept = None
             ctx.save_for_backward(w1, w2, u, x, t)
         else:
-            kx, tx = _keep((x,), slope_in, storage, True)
-            kt, tt = _keep((t,), None, storage, True)
+            need = ctx.needs_input_grad
+            inner = need[0] or any(need[2:6])
+            kx, tx = _keep((x,), slope_in, storage, need[2] or need[3] or need[0] and slope_in is not None)
+            kt, tt = _keep((t,), None, storage, inner)
             ctx.kept = kx + kt
-            ctx.save_for_backward(w1, w2, ops.act_signs(u) if u is not None else None, *tx, *tt)
+            ctx.save_for_backward(w1, w2, ops.act_signs(u) if u is not None and inner else None, *tx, *tt)
         return y
 
     @staticmethod
@@ -197,11 +199,13 @@ class _ResBlock(torch.autograd.Function):
         slope_in, slope_mid, slope_out, pd1, pd2 = ctx.cfg
         dpacked1, dpacked2 = ctx.images
         w1, w2, u, *xt = ctx.saved_tensors
-        x, t = xt if ctx.kept is None else _kept(ctx.kept, xt)
         need = ctx.needs_input_grad
+        g = _rows_ok(g)
+        if not (need[0] or any(need[2:6])):
+            return (None, g) + (None,) * 16
+        x, t = xt if ctx.kept is None else _kept(ctx.kept, xt)
         n, ch, h, w = x.shape
         mid = w1.shape[0]
-        g = _rows_ok(g)
         # second convolution
         if slope_out is None and g.is_contiguous():
             g2 = g
@@ -349,7 +353,7 @@ class _SEGate(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, fc1, fc2, storage):
-        ctx.shape, ctx.means = x.shape, storage is not None
+        ctx.shape, ctx.means = x.shape, storage is not None and any(ctx.needs_input_grad)
         ctx.save_for_backward(ops.plane_dot(x) if ctx.means else x, fc1, fc2)
         return ops.se_gate(x, fc1, fc2)
 
