@@ -790,3 +790,42 @@ def test_weight_gradient_of_one_huge_sample():
     got = ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x), grad, (64, 64, 1, 1)).view(64, 64)
     want = grad.view(64, -1).double() @ x.view(64, -1).double().t()
     assert torch.equal(got.double(), want)
+
+
+def step_gradients(seeded_sd, storage, recompute=False, size=128):
+    """One training step's gradients of the model with its seeded weights, the same noise every time."""
+    from deepvideocodec_amd import train as TR
+    from deepvideocodec_amd.models import DMC
+    from deepvideocodec_amd.testing import synthetic_gop
+    frames = [f.cuda() for f in synthetic_gop(3, size, size, seed=3, batch=2)]
+    net = DMC()
+    net.load_state_dict(seeded_sd)
+    net = net.cuda().train().set_act_storage(storage)
+    net.recompute = recompute
+    torch.manual_seed(5)
+    TR.RateDistortionLoss(lmbda=2048.0)(net(list(frames)), frames[1:])["loss"].backward()
+    return {n: p.grad.double() for n, p in net.named_parameters() if p.grad is not None}
+
+
+@pytest.mark.parametrize("fmt,most", [("int8", 0.1), ("e4m3", 0.15)])
+def test_training_step_gradients_stay_close_to_those_of_fp32_storage(seeded_sd, fmt, most):
+    """Every parameter's gradient against that of fp32 storage.  A stored operand's rounding is independent of the gradient it is
+    multiplied with, so a weight gradient moves by the rounding's root mean square in units of the operand's: int8, half a
+    step below 1/127 of the block's largest, which is at most sqrt(32) of its root mean square: sqrt(32) / 127 / sqrt(3) = 0.026;
+    e4m3, half a step at most 2^-4 of the value: 2^-4 / sqrt(3) = 0.036.  Four times that is allowed, as products and
+    operands are not quite uncorrelated; a wrong mask, scale or layout in any layer is off by the order of one."""
+    want, got = step_gradients(seeded_sd, "fp32"), step_gradients(seeded_sd, fmt)
+    assert want.keys() == got.keys()
+    off = {n: float((got[n] - want[n]).norm() / want[n].norm()) for n in want if float(want[n].norm()) > 0}
+    worst = sorted(off, key=off.get)[-3:]
+    print(fmt, [(n, f"{off[n]:.1e}") for n in worst], f"median {sorted(off.values())[len(off) // 2]:.1e}")
+    assert len(off) > 200 and off[worst[-1]] <= most
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_recompute_with_8_bit_storage_gives_the_same_gradients(seeded_sd, fmt):
+    """Recomputed blocks are stored from the same activations: the same gradients up to the order of sums (and the warp's
+    atomics), as in fp32."""
+    want, got = (step_gradients(seeded_sd, fmt, recompute, 64) for recompute in (False, True))
+    assert want.keys() == got.keys()
+    assert max(float((want[n] - got[n]).abs().max()) / max(float(want[n].abs().max()), 1e-20) for n in want) < 1e-4
