@@ -633,6 +633,12 @@ def _on_current_device(t: Tensor, name: str):
         raise ValueError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _sizes_fit(shape, name: str):
+    """The library takes sizes as 32-bit integers, into which ctypes would wrap a larger one without a word."""
+    if max(shape) >> 31:
+        raise ValueError(f"{name}: shape {tuple(shape)}, every size must be below 2^31")
+
+
 def _ckpt_format(fmt: str) -> int:
     if fmt not in _lib.CKPT_FORMATS:
         raise ValueError(f"unknown checkpoint format {fmt!r} (one of {', '.join(_lib.CKPT_FORMATS)})")
@@ -646,6 +652,7 @@ def _ckpt(ck: ActCheckpoint, name: str, device=None) -> DvcCkpt:
     fmt = _ckpt_format(fmt)
     if n < 1 or c < 1 or h < 1 or w < 1:
         raise ValueError(f"{name}: empty shape {tuple(ck.shape)}")
+    _sizes_fit(ck.shape, name)
     blocks = n * c * ((h * w + 31) // 32)
     _check_vec(codes, blocks * 32, f"{name} codes" if device is not None else name, dtype=torch.uint8, device=device)
     _check_vec(scales, blocks, name, dtype=torch.uint8, device=codes.device)
@@ -676,6 +683,7 @@ def act_checkpoint(x: Tensor, slope: Optional[float] = None, fmt: str = "int8") 
     code = _ckpt_format(fmt)
     src = _src(x, "act_checkpoint x")
     _on_current_device(x, "act_checkpoint x")
+    _sizes_fit(x.shape, "act_checkpoint x")
     n, c, h, w = x.shape
     blocks = (h * w + 31) // 32
     codes = x.new_empty((n, c, blocks * 32), dtype=torch.uint8)
@@ -708,6 +716,7 @@ def act_signs(x: Tensor) -> Tensor:
     """One bit per value, x > 0, as int32 words of 32 adjacent values of a channel plane: (N, C, blocks)."""
     src = _src(x, "act_signs x")
     _on_current_device(x, "act_signs x")
+    _sizes_fit(x.shape, "act_signs x")
     n, c, h, w = x.shape
     signs = torch.empty((n, c, _blocks(h, w)), dtype=torch.int32, device=x.device)
     check(_lib.load().dvc_act_signs(C.byref(src), signs.data_ptr(), n, h, w, _stream()), "dvc_act_signs")
@@ -722,6 +731,7 @@ def act_grad_signs(grad: Tensor, signs: Tensor, slope: float, pixel_shuffle: boo
         raise ValueError(f"act_grad_signs: grad shape {tuple(grad.shape)} != {stored}")
     src = _src(grad, "act_grad_signs grad")
     _on_current_device(grad, "act_grad_signs grad")
+    _sizes_fit(grad.shape, "act_grad_signs grad")
     _check_vec(signs, n * stored[1] * _blocks(*stored[2:]), "act_grad_signs signs", dtype=torch.int32, device=grad.device)
     out = torch.empty((n, c, ho, wo), dtype=torch.float32, device=grad.device)
     check(_lib.load().dvc_act_grad_signs(C.byref(src), signs.data_ptr(), float(slope), 1 if pixel_shuffle else 0,
@@ -819,6 +829,7 @@ def _logits(logits: Tensor, symbols: Tensor, name: str):
         raise ValueError(f"{name}: symbols {tuple(site)} do not match logits {tuple(shape)}")
     _check_vec(symbols, None, name, dtype=torch.int32, device=logits.device)
     _on_current_device(logits, name)
+    _sizes_fit(shape, f"{name} logits")
     if n * h * w == 0:
         return None, n, groups, h, w, rows
     return DvcLogits(logits.data_ptr(), strides[0], strides[1] if shape[1] > 1 else h * w, groups, v, dtype, 0), n, groups, h, w, rows

@@ -491,6 +491,21 @@ def test_refusals_of_the_python_surface():
     ops.act_restore(ck, out=torch.empty(4, 2, 8, 8, device="cuda").transpose(0, 1))      # interleaved samples do not
 
 
+def test_sizes_past_32_bits_are_refused():
+    """A size of 2^31 or more does not fit the library's arguments: refused, not wrapped, and before anything is allocated."""
+    from deepvideocodec_amd import ops
+    x = torch.zeros(1, 1, 4, 4, device="cuda")
+    for shape in (((1 << 32) + 2, 1, 4, 4), (1, (1 << 32) + 2, 4, 4), (1 << 31, 1, 4, 4)):
+        view = x.expand(shape)
+        for call in (lambda: ops.act_checkpoint(view), lambda: ops.act_signs(view),
+                     lambda: ops.act_grad_signs(view, torch.zeros(1, dtype=torch.int32, device="cuda"), 0.1, False, shape),
+                     lambda: ops.mul_act_grad_ckpt(view, ops.act_checkpoint(x)._replace(shape=shape), 0.1, out=view),
+                     lambda: ops.act_restore(ops.act_checkpoint(x)._replace(shape=shape)),
+                     lambda: ops.conv2d_wgrad_ckpt(ops.act_checkpoint(x)._replace(shape=shape), x, (1, shape[1], 3, 3))):
+            with pytest.raises(ValueError):
+                call()
+
+
 def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
     from deepvideocodec_amd import ops
     x = torch.randn(2, 4, 8, 8, device="cuda")

@@ -636,3 +636,16 @@ def test_categorical_rate_behind_checkpointed_layers(fmt):
     # (108 + 640 + 128) 2^-23 = 1.05e-4
     for got, want in ((dev[0].grad, gx), (dev[1].grad, gw1), (dev[2].grad, gb1), (dev[3].grad, gw2), (dev[4].grad, gb2)):
         assert float((got.cpu().double() - want).abs().max()) <= 1.1e-4 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("place,site", [((1, (1 << 32) + 5), (1,)), ((1, 1 << 31), (1,)), ((1, (1 << 32) + 6, 1, 1), (1, 2, 1, 1))])
+def test_sizes_past_32_bits_are_refused(place, site):
+    """A size of 2^31 or more does not fit the library's arguments: refused, not wrapped."""
+    from deepvideocodec_amd import autograd as A, ops
+    x, s = torch.zeros(place, dtype=torch.bfloat16, device="cuda"), torch.zeros(site, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.symbol_log_probs(x, s)
+    with pytest.raises(ValueError, match="2\\^31"):
+        A.symbol_log_probs(x.requires_grad_(), s)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.symbol_log_probs_backward(x.detach(), s, torch.zeros((2, s.numel()), device="cuda"), torch.zeros(s.numel(), device="cuda"), None, None)
