@@ -3,12 +3,16 @@
 //
 // Arithmetic.  The scale of a block of 32 values is a power of two taken from the exponent and mantissa bits of the
 // block's largest magnitude, so x / scale is exact and a code differs from its value only by the one rounding to 7 bits
-// (int8) or 4 significant bits (e4m3): half a step, <= 2^-8 of the block's maximum for int8 (the power of two costs up
-// to one bit against a free scale; it buys exact bf16 operands in the weight gradient), 2^-4 of the value for e4m3.
+// (int8) or 4 significant bits (e4m3).  int8: half a step, which is 1/254 to 1/127 of the block's maximum (the power of two
+// costs up to one bit against a free scale; it buys exact bf16 operands in the weight gradient).  e4m3: 2^-4 of the value,
+// or 2^-10 of the block's scale where that is more (values below 2^-6 scales, 2^-14 to 2^-15 of the maximum).
 //
 // All kernels are bound by HBM: 4 + 33/32 bytes per value to store or restore.  One lane handles a unit of 4 adjacent
 // values (one 16-byte access), 8 lanes a block (maximum by three lane swaps), a workgroup 4 x 256 units (four
 // requests in flight per lane).  A workgroup's first plane is found once; a lane adds its local offset to that.
+// 32x64x256x256: store 138 us of 125 (at 5.4 TB/s), restore 119 of 125, signs 99 of 103; planes whose rows are no multiple of
+// four take four dword accesses a lane: reading them costs nothing (store at 255x253 132 us), writing them doubles the time
+// (restore 252, sign-only adjoints 331-436 of 199-318).
 #include "dvc_common.h"
 
 namespace {

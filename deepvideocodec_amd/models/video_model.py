@@ -675,9 +675,10 @@ class DMC(nn.Module):
     def set_act_storage(self, storage: str = "fp32"):
         """What the tape of a training step keeps of the convolutions' operands: "fp32" (default) the tensors
         themselves; "int8" or "e4m3" 8-bit checkpoints with one power-of-two scale per 32 adjacent values of a channel
-        plane, and one bit per value where only an activation's derivative is needed.  The forward pass and the data and
-        bias gradients do not change; a weight gradient is that of the stored operand (int8: off by at most half of
-        1/127..1/63 of the block's largest magnitude, e4m3: by at most 1/16 of each value)."""
+        plane, and one bit per value where only an activation's derivative is needed.  The forward pass does not change; a
+        weight gradient is that of the stored operand (int8: off by half a step at most, 1/254..1/127 of the block's largest
+        magnitude; e4m3: by 1/16 of the value, or 2^-10 of the block's scale where that is more), and so is a
+        squeeze-excite gate's; data and bias gradients do not change but for what comes through such a gate."""
         if storage != "fp32" and storage not in _lib.CKPT_FORMATS:
             raise ValueError(f"unknown activation storage {storage!r} (fp32, {', '.join(_lib.CKPT_FORMATS)})")
         for m in self.modules():

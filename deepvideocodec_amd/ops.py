@@ -677,9 +677,10 @@ def _slope(slope: float, name: str) -> float:
 
 
 def act_checkpoint(x: Tensor, slope: Optional[float] = None, fmt: str = "int8") -> ActCheckpoint:
-    """The 8-bit checkpoint of x, or of LeakyReLU(slope)(x) (0.0: ReLU), in `fmt`: "int8" (127 steps of the block's
-    largest magnitude) or "e4m3" (4 significant bits each).  act_restore() gives the values back; the weight gradient
-    (conv2d_wgrad_ckpt) and the input activation's derivative (mul_act_grad_ckpt) read the codes themselves."""
+    """The 8-bit checkpoint of x, or of LeakyReLU(slope)(x) (0.0: ReLU), in `fmt`: "int8" (64 to 127
+    steps up to the block's largest magnitude) or "e4m3" (4 significant bits each, down to 2^-14 of it).  act_restore() gives
+    the values back; the weight gradient (conv2d_wgrad_ckpt) and the input activation's derivative (mul_act_grad_ckpt) read
+    the codes themselves."""
     code = _ckpt_format(fmt)
     src = _src(x, "act_checkpoint x")
     _on_current_device(x, "act_checkpoint x")
@@ -841,8 +842,9 @@ def symbol_log_probs(logits: Tensor, symbols: Tensor, top: int = 0) -> SymbolLog
 
     logits (N, C * classes, h, w), symbols (N, C, h, w) int32: channel c's classes are the channels c * classes ...;
     or rows, logits (N, classes), symbols (N,).  fp32, bf16 or fp16 logits with free batch and class strides; sums are
-    fp32.  A symbol < 0 means "none here" (log probability 0); one past the last class gives NaN.  Classes that may not
-    occur have logits of -inf; a site without any other has log probability -inf and entropy 0."""
+    fp32 (over more than 256 classes a lane of the GPU, 64 bits).  A symbol < 0 means "none here" (log probability 0); one
+    past the last class gives NaN.  Classes that may not occur have logits of -inf; a site without any other has log
+    probability -inf and entropy 0.  Rows of more than 1024 classes: below 2^24 of them, of more than 256: below 2^26."""
     lg, n, groups, h, w, rows = _logits(logits, symbols, "symbol_log_probs")
     classes = logits.size(1) // groups
     top = int(top)

@@ -404,7 +404,8 @@ int dvc_mul_act_grad_ckpt(const DvcSrc* grad, const DvcCkpt* x, float slope, con
 /* dvc_conv2d_wgrad with the sources given by checkpoints of their activated values (all of one format).
  * Deterministic; scratch starts on 16 bytes.  The products are exact: a code times its power of two is a bf16 number, and the gradient is split
  * into three bf16 parts that add up to it; sums are fp32.  (A block that restores to NaN, or a gradient that is not
- * finite, reaches every weight it takes part in as NaN.) */
+ * finite, reaches every weight it takes part in as NaN.)  The scratch does not grow with the pixels: 128 MiB, or one 64 x 64
+ * (7x7: 32 x 32) block of every tap for each of 256 workgroups or 64 x 64 weights where that is more, and the bias sums. */
 int64_t dvc_conv2d_wgrad_ckpt_scratch_floats(int32_t cout, int32_t cin, int32_t ksize, int32_t stride,
                                              int32_t batch, int32_t in_h, int32_t in_w);
 int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t batch, int32_t in_h, int32_t in_w,
@@ -423,6 +424,9 @@ int dvc_conv2d_wgrad_ckpt(const DvcCkpt* srcs, int32_t n_src, int32_t batch, int
  *   exp(logit - max)): what dvc_symbol_log_probs_backward needs.
  *   top (0..DVC_MAX_TOP, <= classes): the `top` most likely classes in falling order (equal logits: the lower class
  *   first, NaN above all), as log probabilities and classes, contiguous (batch, groups * top, h, w).
+ * Refused: more rows (h*w = 1, adjacent classes) than one launch has threads for -- 2^24 above 1024 classes, of the gradient
+ * 2^24 rows times 16-kB pieces, 2^26 above 256 classes, 2^29 above 128 -- and 2^31 groups or
+ * 2^32 sites of any kind.
  */
 #define DVC_MAX_TOP 16
 #define DVC_F32 0
