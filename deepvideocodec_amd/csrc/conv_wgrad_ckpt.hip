@@ -9,9 +9,9 @@ int launch_aligned(int ks, int stride, const Args& a, const Plan& p, hipStream_t
 namespace {
 
 // gW[co][ci][tap] = sum over slabs of partial[slab][tap][co][ci], gB[co] likewise over splits (units past the weight's); `more`: added
-// to what they hold.  A lane
-// takes four adjacent input channels (rows of a slab are padded to 32), a block UNITS such units; each of its GROUPS groups of
-// lanes adds every GROUPS-th slab, with the loads of four slabs in flight, and the sums are added in a fixed order.
+// to what they hold.  A lane takes four adjacent input channels (rows of a slab are padded to 32), a block UNITS such units; each
+// of its GROUPS groups of lanes adds every GROUPS-th slab, with the loads of four slabs in flight, and the sums are added in a
+// fixed order.
 __device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
 template <int UNITS, int GROUPS>
