@@ -326,7 +326,7 @@ def wgrad64_gpu(x, g, k, stride):
 
 
 @pytest.mark.parametrize("k,cin,cout,h,w,batch", [
-    (3, 192, 192, 256, 256, 6),      # 3072 tiles over 29 workgroups a block: four slabs in time, two launches of two
+    (3, 192, 192, 256, 256, 6),      # 106 tiles for each of 29 workgroups a block: four slabs in time, two launches of two
     (3, 192, 160, 256, 253, 7),      # five: of three and two
     (7, 64, 64, 42, 4740, 5),        # 8195 tiles over 64 workgroups: three slabs, in the second launch three tiles
     (7, 64, 64, 42, 4739, 5),
@@ -377,8 +377,8 @@ def real_sums(k, stride, cin, cout, h, w, batch, fmt):
     (3, 1, 192, 192, 256, 256, 8, "e4m3")])
 def test_weight_gradient_of_long_sums_of_real_numbers(k, stride, cin, cout, h, w, batch, fmt):
     """All three parts of the gradient arrive in every form and at every place of a tile.  A slab is at most 512 row pieces of
-    three matrix instructions that round twice: 3072 roundings of a sum that grows like a random walk, 2^-24 / sqrt(3) of
-    its size each, come to sqrt(3072 / 2) 2^-24 / sqrt(3) = 1.4e-6 of the result.  Without the third part every gradient is
+    three matrix instructions that round twice: n = 6 x 512 roundings of a sum that grows like a random walk, 2^-24 / sqrt(3)
+    of its size each, come to sqrt(n / 2) 2^-24 / sqrt(3) = 1.4e-6 of the result.  Without the third part every gradient is
     cut off by 2^-17 (5.5e-6 on average, all towards zero); without the second by 2^-9."""
     assert float(real_sums(k, stride, cin, cout, h, w, batch, fmt).square().mean().sqrt()) <= 3e-6
 
